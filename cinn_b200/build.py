@@ -30,6 +30,7 @@ SOURCES = [
     "ew_stream.cu",
     "reduce_static_scratch.cu",
     "peer_reduce.cu",
+    "row_loss.cu", "router_loss.cu", "loss_ops.cc",
     "group_desc.cc",
     "group_match.cc",
     "chain_match.cc",

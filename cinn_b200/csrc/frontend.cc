@@ -13,6 +13,7 @@
 #include <sstream>
 
 #include "../../include/cinn_b200.h"
+#include "loss_ops.h"
 
 namespace cinn_b200 {
 
@@ -112,7 +113,7 @@ bool KnownOp(const std::string& t) {
   return UnaryOps().count(t) || BinaryOps().count(t) || CompareOps().count(t) || ReduceOps().count(t) ||
          t == "scale" || t == "cast" || t == "select" || t == "broadcast_to" || t == "fill_constant" ||
          t == "softmax" || t == "batch_norm" || t == "reshape" || t == "squeeze" || t == "expand_dims" ||
-         t == "transpose" || t == "slice" || t == "concat";
+         t == "transpose" || t == "slice" || t == "concat" || t == "balance_loss" || IsLossOp(t);
 }
 
 bool IsBinaryBroadcastOp(const std::string& t) { return BinaryOps().count(t) || CompareOps().count(t); }
@@ -124,6 +125,8 @@ OpPattern PatternOf(const std::string& t) {
   if (t == "reshape") return OpPattern::kNonFusible;
   // Data movement (registered kInjective in the reference, cinn/hlir/op/transform.cc): a kernel of its own here.
   if (t == "transpose" || t == "slice" || t == "concat") return OpPattern::kNonFusible;
+  // A loss op fuses with the other loss ops over its logits and with nothing else (a step of its own in FusePasses).
+  if (IsLossOp(t)) return OpPattern::kNonFusible;
   // softmax is registered kNonFusible in the reference (cinn/hlir/op/nn.cc:2383-2393); here the casts around
   // it may join its group, so it takes part in fusion like an elementwise op.
   return OpPattern::kElementWise;
@@ -210,8 +213,29 @@ int NetBuilder::AddOp(const std::string& op, const std::vector<int>& inputs,
     }
     return AddOp("reshape", inputs, {{"shape", JoinInts(shape)}}, err);
   }
+  if (op == "balance_loss") {
+    // Column sums of the routing probabilities, then one number from them: two instructions, the first of which shares
+    // its pass over the logits with balance_loss_grad.
+    if (!need(3)) return fail("takes 3 inputs (logits, counts, weight)");
+    const int load = AddOp("expert_load", {inputs[0], inputs[2]}, {}, err);
+    return load < 0 ? -1 : AddOp("balance_fold", {load, inputs[1]}, {}, err);
+  }
   Variable out;
-  if (UnaryOps().count(op)) {
+  if (IsLossOp(op)) {
+    std::vector<TensorDesc> descs;
+    for (size_t k = 0; k < inputs.size(); ++k) {
+      TensorDesc t;
+      t.name  = in(k).id;
+      t.dtype = in(k).dtype;
+      t.shape = in(k).shape;
+      descs.push_back(t);
+    }
+    TensorDesc result;
+    std::string e;
+    if (!InferLossOp(op, descs, &attrs, &result, &e)) return fail(e);
+    out.dtype = result.dtype;
+    out.shape = result.shape;
+  } else if (UnaryOps().count(op)) {
     if (!need(1)) return fail("takes 1 input");
     out.dtype = PredicateOps().count(op) ? DType::kBool : in(0).dtype;
     out.shape = in(0).shape;
@@ -971,6 +995,26 @@ bool FusePasses(const NetBuilder& b, const std::vector<int>& fetch_in, const Dev
         sets[j].clear();
         break;  // a group has two outputs at most
       }
+    }
+  }
+
+  // Step 4b: the loss ops over one tensor of logits (a loss, its gradient, the log-probabilities) become one group when
+  // a kernel takes them together: the logits are then read once.
+  for (size_t i = 0; i < sets.size(); ++i) {
+    auto only_loss_ops = [&](const std::set<int>& m) {
+      for (int k : m)
+        if (!IsLossOp(b.instrs()[k].op_type)) return false;
+      return !m.empty();
+    };
+    if (!only_loss_ops(sets[i])) continue;
+    for (size_t j = i + 1; j < sets.size(); ++j) {
+      if (!only_loss_ops(sets[j]) || b.instrs()[*sets[i].begin()].inputs[0] != b.instrs()[*sets[j].begin()].inputs[0]) continue;
+      std::set<int> merged = sets[i];
+      merged.insert(sets[j].begin(), sets[j].end());
+      if (leaves_and_reenters(merged) || !st.Compiles(merged, nullptr, nullptr)) continue;
+      for (int k : sets[j]) group_of[k] = (int)i;
+      sets[i] = merged;
+      sets[j].clear();
     }
   }
 

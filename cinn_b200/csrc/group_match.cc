@@ -14,6 +14,7 @@
 #include <sstream>
 
 #include "group_desc.h"
+#include "loss_ops.h"
 
 namespace cinn_b200 {
 
@@ -1607,6 +1608,8 @@ struct Matcher {
 
 std::unique_ptr<CompiledGroup> CompileGroup(const GroupDesc& g, const DeviceInfo& dev, std::string* err) {
   std::string local;
+  for (auto& op : g.ops)
+    if (IsLossOp(op.type)) return MatchLossGroup(g, dev, err ? err : &local);
   Matcher m(g, dev, err ? err : &local);
   return m.Run();
 }

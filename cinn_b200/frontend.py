@@ -386,6 +386,64 @@ class NetBuilder:
                      self.broadcast_to(beta, [rows, cols], [1]))
         return self.cast(y, dt) if half else y
 
+    # ---- losses over rows of logits, and their gradients ------------------------------------------------
+    # `logits` is [rows..., columns] in float32 / float16 / bfloat16; ids are int32 / int64; everything with one value
+    # per row (rows...) is float32.  A row whose `weight` is 0 is out: loss 0 and a gradient row of zeros, whatever
+    # else it holds.  `weight` (and `dlogprob`) may be a fill_constant.  A gradient is that of the SUM of the losses;
+    # scale it through the weight.  The ops over one tensor of logits run as one kernel that reads it once.
+    def token_logprob(self, logits, target, temperature=1.0):
+        """log softmax(logits / temperature)[target], float32; 0 where the target lies outside [0, columns)."""
+        return self._op("token_logprob", [logits, target], temperature=float(temperature))
+
+    def token_logprob_grad(self, logits, target, dlogprob, temperature=1.0):
+        """Gradient of token_logprob with respect to the logits, given its upstream gradient (-1 / rows in every row
+        for a mean cross entropy): dlogprob / temperature * (onehot(target) - softmax)."""
+        return self._op("token_logprob_grad", [logits, target, dlogprob], temperature=float(temperature))
+
+    def policy_loss(self, logits, action, old_logprob, ref_logprob, advantage, weight, clip_low=0.2, clip_high=0.2,
+                    kl_coef=0.0, temperature=1.0):
+        """Clipped policy loss per token, with the KL term against a reference policy: with lp = log
+        softmax(logits / temperature)[action], r = exp(lp - old_logprob) and gap = ref_logprob - lp,
+        weight * (kl_coef * (exp(gap) - gap - 1) - min(r * advantage, clip(r, 1 - clip_low, 1 + clip_high) * advantage)).
+        With kl_coef 0 the reference's log-probabilities are not read.  float32."""
+        return self._op("policy_loss", [logits, action, old_logprob, ref_logprob, advantage, weight],
+                        clip_low=float(clip_low), clip_high=float(clip_high), kl_coef=float(kl_coef),
+                        temperature=float(temperature))
+
+    def policy_loss_grad(self, logits, action, old_logprob, ref_logprob, advantage, weight, clip_low=0.2, clip_high=0.2,
+                         kl_coef=0.0, temperature=1.0):
+        """Gradient of the sum of policy_loss with respect to the logits, in their type."""
+        return self._op("policy_loss_grad", [logits, action, old_logprob, ref_logprob, advantage, weight],
+                        clip_low=float(clip_low), clip_high=float(clip_high), kl_coef=float(kl_coef),
+                        temperature=float(temperature))
+
+    def distill_loss(self, logits, teacher_logits, teacher_index, weight, temperature=1.0):
+        """Divergence of the student's softmax from a teacher known by its top logits: [rows..., entries] logits and
+        the columns they belong to (outside [0, columns): an unused entry; a column may occur more than once).  With
+        p = softmax over the row's used entries of teacher_logits / temperature and q = softmax(logits / temperature),
+        weight * sum_k p_k (log p_k - log q[index_k]) per row, float32.  At most 1024 entries."""
+        return self._op("distill_loss", [logits, teacher_logits, teacher_index, weight], temperature=float(temperature))
+
+    def distill_loss_grad(self, logits, teacher_logits, teacher_index, weight, temperature=1.0):
+        """Gradient of the sum of distill_loss with respect to the student's logits, in their type."""
+        return self._op("distill_loss_grad", [logits, teacher_logits, teacher_index, weight],
+                        temperature=float(temperature))
+
+    def expert_counts(self, index, weight, num_experts):
+        """How often each expert was chosen: `index` [tokens..., slots] holds the chosen experts, an entry outside
+        [0, num_experts) and every entry of a token of weight 0 is not counted.  int32 [num_experts], at most 1024."""
+        return self._op("expert_counts", [index, weight], num_experts=int(num_experts))
+
+    def balance_loss(self, logits, counts, weight):
+        """Load-balance loss of a router: with f = counts / sum(counts) and q = softmax(logits) over the experts (the
+        last axis, at most 1024), experts * sum_e f_e sum_t weight_t q_te; float32 [1].  `counts` is a constant of the
+        differentiation; with several replicas, pass the counts of all of them."""
+        return self._op("balance_loss", [logits, counts, weight])
+
+    def balance_loss_grad(self, logits, counts, weight):
+        """Gradient of balance_loss with respect to the router's logits, in their type."""
+        return self._op("balance_loss_grad", [logits, counts, weight])
+
 
 class Tensor:
     """A tensor of a computation's scope (hlir::framework::Tensor as exposed by cinn/pybind/framework.cc:116-172)."""
