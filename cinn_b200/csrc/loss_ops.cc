@@ -15,6 +15,7 @@ constexpr int64_t kMaxTeacherEntries = 1024;  // entries per row that distill_lo
 constexpr int64_t kMaxExperts        = 1024;  // a warp keeps a router row of this length in registers
 
 int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t RoundUp(int64_t a, int64_t b) { return CeilDiv(a, b) * b; }
 
 bool IsLogits(DType t) { return t == DType::kFloat32 || t == DType::kFloat16 || t == DType::kBFloat16; }
 bool IsIndex(DType t) { return t == DType::kInt32 || t == DType::kInt64; }
@@ -327,7 +328,7 @@ struct LossMatcher {
     const char* kinds[] = {"logprob", "policy", "distill"};
     auto p = NewPlan("row_loss");
     LaunchStep s;
-    const std::string name = std::string("row_loss_") + kinds[kind] + "_" + ShortName(x.dtype);
+    const std::string name = std::string("row_loss_") + kinds[kind] + (grad ? "_grad_" : "_") + ShortName(x.dtype);
     s.kernel = FindKernel(name);
     if (!s.kernel) return Fail("kernel " + name + " is missing");
     auto arg = [&](size_t k) { return In(main.inputs[k]); };
@@ -353,8 +354,24 @@ struct LossMatcher {
     s.args.push_back(weight < 0 ? F(0.0) : Constant(main.inputs[weight]));
     s.args.push_back(F(Attr(main, "temperature")));
     for (const char* key : {"clip_low", "clip_high", "kl_coef"}) s.args.push_back(F(kind == 1 ? Attr(main, key) : 0.0));
-    s.block[0] = 256;
-    s.grid[0]  = (unsigned)std::min<int64_t>(rows, (int64_t)dev.sm_count * 8);
+    return ShapeRows(std::move(p), s, rows, cols * DTypeBytes(x.dtype), 12 * entries, grad != nullptr);
+  }
+
+  // Warps per CTA, CTAs per row and ring slots of the row kernels (row_loss.cu says what was measured).
+  std::unique_ptr<CompiledGroup> ShapeRows(std::unique_ptr<CompiledGroup> p, LaunchStep s, int64_t rows, int64_t row_bytes,
+                                           int64_t kept_bytes, bool grad) {
+    const int64_t vecs = row_bytes / 16 + 1;
+    int64_t warps = 1, ctas = 1;
+    while (warps < 8 && warps * 256 < vecs) warps *= 2;
+    while (ctas < 8 && rows * ctas * 2 <= dev.sm_count && vecs > 32 * warps * ctas) ctas *= 2;
+    int64_t slots = grad && warps == 8 ? 6 : 4;
+    slots         = std::min(slots, CeilDiv(vecs, 128 * warps));
+    if (rows * ctas > 2147483647) return Fail("more than 2^31 - 1 rows");
+    s.args.push_back(I(slots));
+    s.cluster  = ctas > 1 ? (unsigned)ctas : 0;
+    s.dyn_smem = (size_t)(slots * (warps * 2048 + 16) + 8 * warps * ctas + kept_bytes);
+    s.block[0] = (unsigned)(32 * warps + 32);
+    s.grid[0]  = (unsigned)(ctas * rows);
     p->steps.push_back(s);
     return p;
   }

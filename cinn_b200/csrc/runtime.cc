@@ -209,23 +209,23 @@ static int LaunchEntry(const KernelEntry* entry, void* v_args, int num_args, int
   cfg.blockDim         = dim3(bx, by, bz);
   cfg.dynamicSmemBytes = dyn_smem;
   cfg.stream           = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
   if (cluster_x > 1) {
-    attr[0].id               = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster_x;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs                = attr;
-    cfg.numAttrs             = 1;
-  } else if (entry->pdl && g_opt_pdl) {
+    cudaLaunchAttribute& a = attr[cfg.numAttrs++];
+    a.id                   = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x     = cluster_x;
+    a.val.clusterDim.y     = 1;
+    a.val.clusterDim.z     = 1;
+  }
+  if (entry->pdl && g_opt_pdl) {
     // Programmatic dependent launch: the kernel may be scheduled while the previous kernel of the stream is still
     // draining; it blocks in grid_dependency_sync() (griddepcontrol.wait) until that kernel has completed and its
     // writes are visible, so the stream's ordering is kept and only the launch latency is hidden.  Short launches
     // (a shard of a group on one of eight GPUs runs 5-15 us) gain 1-2 us each.
-    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs                                          = attr;
-    cfg.numAttrs                                       = 1;
+    cudaLaunchAttribute& a                       = attr[cfg.numAttrs++];
+    a.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
   }
   cudaError_t e = cudaLaunchKernelExC(&cfg, kernel_fn, params);
   if (e != cudaSuccess)
