@@ -369,7 +369,7 @@ struct LossMatcher {
     if (rows * ctas > 2147483647) return Fail("more than 2^31 - 1 rows");
     s.args.push_back(I(slots));
     s.cluster  = ctas > 1 ? (unsigned)ctas : 0;
-    s.dyn_smem = (size_t)(slots * (warps * 2048 + 16) + 8 * warps * ctas + kept_bytes);
+    s.dyn_smem = (size_t)(slots * (warps * 2048 + 16) + 8 + 8 * warps * ctas + kept_bytes);
     s.block[0] = (unsigned)(32 * warps + 32);
     s.grid[0]  = (unsigned)(ctas * rows);
     p->steps.push_back(s);

@@ -169,6 +169,12 @@ __global__ void __launch_bounds__(1024) k_expert_zero(int* __restrict__ counts, 
   for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[e] = 0;
 }
 
+// All warps of the cluster, each of them together.
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // loss = E / sum c * sum over slices and experts of c_e load_ke: one flat dot product, over the CTAs of one cluster.
 __global__ void __launch_bounds__(1024)
     k_balance_fold(const float* __restrict__ load, const int* __restrict__ counts, float* __restrict__ out,
@@ -207,16 +213,11 @@ __global__ void __launch_bounds__(1024)
   total = cta_allreduce<SumOp>(total, scratch);
   sum = cta_allreduce<SumOp>(sum, scratch);
   if (C > 1) {
-    if (threadIdx.x == 0) {
-      uint32_t there;
-      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(meet + rank)));
-      // no CTA writes to the first one's shared memory before that one runs
-      asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(sum) : "memory");
-    } else {
-      asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-    }
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(meet + rank)));
+    cluster_barrier();  // no CTA writes to the first one's shared memory before that one runs
+    if (threadIdx.x == 0) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(sum) : "memory");
+    cluster_barrier();
     sum = 0.0f;
     if (rank == 0)
       for (int k = 0; k < C; ++k) sum += meet[k];

@@ -186,7 +186,7 @@ __device__ __forceinline__ void policy_terms(float lp, float old, float ref, flo
   const float r = expf(lp - old), free = r * adv, held = fminf(fmaxf(r, c.lo), c.hi) * adv;
   *loss  = -fminf(free, held);
   *slope = free <= held ? -free : 0.0f;
-  if (r != r || adv != adv) *loss = *slope = r * adv;  // fminf drops a NaN
+  if (free != free) *loss = *slope = free;  // fminf drops a NaN
   if (c.kl != 0.0f) {
     const float gap = ref - lp, e = expm1f(gap);  // expm1: gap is near 0 while the policy is near the reference
     *loss += c.kl * (e - gap);
@@ -210,6 +210,12 @@ __device__ __forceinline__ void bulk_load_hint(void* smem_dst, const void* gmem_
                    smem_addr(smem_dst)),
                "l"(gmem_src), "r"(bytes), "r"(smem_addr(bar)), "l"(policy)
                : "memory");
+}
+// All warps of the cluster, each of them together.
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Where a row's vectors lie: `head` elements in front of the first 16-byte boundary, `nvec` vectors, `tail` elements;
 // and this CTA's stretch of the vectors, `count` from `start` on (`per` to a CTA).
@@ -252,7 +258,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
   const long long row = blockIdx.x / C;
   uint64_t* full  = reinterpret_cast<uint64_t*>(smem + (size_t)N * slot_bytes);
   uint64_t* empty = full + N;
-  float2* meet    = reinterpret_cast<float2*>(empty + N);  // [G]
+  uint64_t* met   = empty + N;                             // completes when the pairs of all G warps are here
+  float2* meet    = reinterpret_cast<float2*>(met + 1);    // [G]
   int* kept_id    = reinterpret_cast<int*>(meet + G);      // [entries], the distillation's
   float* kept_t   = reinterpret_cast<float*>(kept_id + entries);
   float* kept_x   = kept_t + entries;
@@ -313,33 +320,33 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], W);
     }
+    mbar_init(met, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (C > 1) mbar_arrive_expect_tx(met, (uint32_t)G * 8u);
     for (int i = 0; i < min(N, total); ++i) copy(i, i);
   }
+  __syncwarp();
   __syncthreads();
-  if (C > 1) {  // no CTA writes to another's shared memory before that one runs
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-  }
+  if (C > 1) cluster_barrier();  // no CTA writes to another's shared memory before that one runs
   if (producer) {
-    if (C > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // has nothing to bring to the meeting
-    if (lane == 0) {
-      bool ok  = true;
-      int made = min(N, total);
-      for (int i = made, s = 0, n = 0; i < total && ok; ++i) {
-        ok = mbar_wait_bounded(&empty[s], n & 1);
-        if (ok) {
+    bool ok  = true;  // (the warp stays together: the barriers of a cluster are passed by warps, not by lanes)
+    int made = min(N, total);
+    for (int i = made, s = 0, n = 0; i < total && ok; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], n & 1));
+      if (ok) {
+        if (lane == 0) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the slot's readers before its refill
           copy(i, s);
-          ++made;
         }
-        if (++s == N) s = 0, ++n;
+        __syncwarp();
+        ++made;
       }
-      // Every copy lands before the warp that issued it leaves.
-      for (int i = max(0, made - N); i < made; ++i) ok = mbar_wait_bounded(&full[i % N], (i / N) & 1) && ok;
-      if (!ok) atomicAdd(&g_row_loss_wait_timeouts, 1u);
+      if (++s == N) s = 0, ++n;
     }
-    if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    // Every copy lands before the warp that issued it leaves.
+    for (int i = max(0, made - N); i < made; ++i) ok = mbar_wait_bounded(&full[i % N], (i / N) & 1) && ok;
+    if (!__all_sync(0xffffffffu, ok) && lane == 0) atomicAdd(&g_row_loss_wait_timeouts, 1u);
+    if (C > 1) cluster_barrier();
     return;
   }
   float xe = -INFINITY, xa = 0.0f, old = 0.0f, ref = 0.0f, adv = 0.0f;
@@ -416,13 +423,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
       asm volatile("bar.sync 1, %0;" ::"r"(T32) : "memory");
     } else {
       if (lane < C) {
-        uint32_t there;
+        uint32_t there, bar;
         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_addr(meet + g)), "r"(lane));
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(t.m), "f"(t.s) : "memory");
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_addr(met)), "r"(lane));
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(there), "l"(pair(t.m, t.s)), "r"(bar)
+                     : "memory");
       }
       __syncwarp();
-      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      if (KIND == kDistill) asm volatile("bar.sync 1, %0;" ::"r"(T32) : "memory");  // the entries above
+      if (!dead && !mbar_wait_bounded(met, 0)) dead = true;
     }
     Sum u = {-INFINITY, 0.0f};
     for (int n = lane; n < G; n += 32) {
@@ -525,6 +534,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
     }
   }
   if (__any_sync(0xffffffffu, dead) && lane == 0) atomicAdd(&g_row_loss_wait_timeouts, 1u);
+  if (C > 1) cluster_barrier();  // no CTA leaves while another may still write to its shared memory
 }
 
 }  // namespace

@@ -295,6 +295,32 @@ def test_balance_loss_its_gradient_and_the_counts(rows, experts, k, dtype):
     check_grad(got["dx"], grad, parts, d, "dlogits")
 
 
+@pytest.mark.parametrize("rows,cols", [(60, 131072), (2, 1000003), (20, 150001)])
+def test_few_rows_too_long_for_the_rings_of_their_ctas(rows, cols):
+    """Several CTAs share such a row, and each brings its part in twice."""
+    g, x, a = make(rows, cols, "bfloat16")
+    p, t = policy_inputs(g, x, a), distill_inputs(g, x, 70)
+    inputs = {**p, "t": t["t"], "i": t["i"]}
+    want, second = policy64(*p.values(), 0.2, 0.28, 0.05, 1.0), distill64(x, t["t"], t["i"], p["w"], 1.0)
+
+    def build(b, v):
+        args = [v[k] for k in ("x", "a", "old", "ref", "adv", "w")]
+        return {"lp": b.token_logprob(v["x"], v["a"]), "dx": b.policy_loss_grad(*args, **POLICY),
+                "dl": b.distill_loss(v["x"], v["t"], v["i"], v["w"]), "ddx": b.distill_loss_grad(v["x"], v["t"], v["i"], v["w"])}
+    got = run_program(build, inputs)
+    alone = run_program(lambda b, v: {"lp": b.token_logprob(v["x"], v["a"])}, inputs)
+    d = delta(x, 1.0)
+    off = d + 8 * U * (want["logprob"].abs() + 1)
+    near(got["lp"], want["logprob"], off, "logprob")
+    near(alone["lp"], want["logprob"], off, "logprob alone")
+    hot = torch.softmax(x.double(), -1).scatter_add(1, a.long()[:, None], torch.ones(rows, 1, dtype=torch.float64, device="cuda"))
+    tol = (d * want["slope"] + want["steep"] * off + 16 * U * want["terms"])[:, None] * hot
+    near(got["dx"], want["dlogits"], half_step(x.dtype) * want["dlogits"].abs() * 1.001 + 1.01 * tol + tiniest(x.dtype), "dlogits")
+    d = d + delta(t["t"], 1.0) + 16 * U
+    near(got["dl"], second["loss"], 2 * d * second["size"], "distill")
+    check_grad(got["ddx"], second["dlogits"], p["w"].double()[:, None] * (second["q"] + second["mass"]), d[:, None], "distill dlogits")
+
+
 # ---- rows that are out, masks, borders ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("cols", [37, 4096, 40009])
