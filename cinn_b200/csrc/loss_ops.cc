@@ -364,8 +364,7 @@ struct LossMatcher {
     int64_t warps = 1, ctas = 1;
     while (warps < 8 && warps * 256 < vecs) warps *= 2;
     while (ctas < 8 && rows * ctas * 2 <= dev.sm_count && vecs > 32 * warps * ctas) ctas *= 2;
-    int64_t slots = grad && warps == 8 ? 6 : 4;
-    slots         = std::min(slots, CeilDiv(vecs, 128 * warps));
+    const int64_t slots = std::min<int64_t>(4, CeilDiv(vecs, 128 * warps));
     if (rows * ctas > 2147483647) return Fail("more than 2^31 - 1 rows");
     s.args.push_back(I(slots));
     s.cluster  = ctas > 1 ? (unsigned)ctas : 0;

@@ -18,17 +18,17 @@
 // and one whose first lane brings the row's 16-byte vectors through a ring of N shared-memory slots (four vectors per
 // computing thread each) with bulk asynchronous copies.  Pass 1 keeps a running reference and sum per lane; the warps'
 // (reference, sum) pairs meet once, in shared memory or in distributed shared memory across the cluster.  Pass 2 turns
-// the row into its gradient: from the ring when the whole row fits it, otherwise the row comes through the ring again,
-// from L2, its first copies on their way while the pairs meet.  Copies of pass 1 ask L2 to keep the row (evict_last),
-// copies of pass 2 let it go (evict_first).  CTAs are not persistent: the hardware deals rows to SMs as they come free,
-// which rows that are out make uneven, and co-resident CTAs cover one another's ends.
+// the row into its gradient: first the last chunks, which are still in the ring, then the others, which come through
+// the ring again from L2, the last one first.  Copies that will be wanted again ask L2 to keep them (evict_last), the
+// others let go (evict_first).  CTAs are not persistent: the hardware deals rows to SMs as they come free, which rows
+// that are out make uneven, and co-resident CTAs cover one another's ends.
 //
-// Measured on 4096 x 131072 bf16 logits (of the measured copy bandwidth): the log-probability alone 0.97 (168 us), with
-// its gradient 0.90 (363 us).  Without the L2 hints half of pass 2's reads miss L2: 0.76.  Rings of 6 / 4 / 3 slots of 8
-// warps: 0.90 / 0.77 / 0.77 with the gradient, of 4 / 3 slots 0.98 / 0.97 without; 16 warps x 4 slots 0.78, 4 warps x 8
-// slots 0.76.  The row held on chip by a cluster of 2 or 4 CTAs: 0.68 (the cluster's barrier stops all its SMs at once).
-// Persistent CTAs that fetch the next row ahead, with a ring per warp: 0.75 (0.85 without the gradient).  Plain loads
-// into registers: 0.81 and 0.83.
+// Measured on 4096 x 131072 bf16 logits, single launches / back to back at the power cap, of the measured copy bandwidth:
+// the log-probability alone 0.97 / 0.92, with its gradient 0.90 / 0.84.  Without the L2 hints half of pass 2's reads miss L2:
+// 0.76.  4 slots of 8 warps against 3 / 6 slots: level on long rows, 0.64 against 0.64 / 0.55 at 1000 x 50021 fp16; 16 warps
+// 0.78, 4 warps 0.80.  Pass 2 without the chunks that are still there 0.825.  The row held on chip by a cluster of 2 or 4
+// CTAs: 0.68; rings in clusters of 2 / 4: 0.80 / 0.74.  Persistent CTAs that fetch the next row ahead, rows dealt statically
+// or by cluster launch control: 0.75, 0.77.  Plain loads into registers: 0.81.
 //
 // Every wait on a copy is bounded: a warp that gives up records it (cinn_b200_device_status) and goes on through the
 // barriers it shares with others; the copying lane waits for all its copies, bounded, before it leaves.
@@ -305,11 +305,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
 
   const int chunk  = T32 * kUnroll;                               // vectors of a slot
   const int chunks = (r.count + chunk - 1) / chunk;
-  const bool held  = GRAD && chunks <= N;                         // pass 2 finds the row in the ring
-  const int total  = GRAD && !held ? 2 * chunks : chunks;
+  const int held   = GRAD ? min(chunks, N) : 0;                   // pass 2 finds the last ones still in the ring
+  const int total  = GRAD ? 2 * chunks - held : chunks;           // and has the others fetched again, last one first
   const bool producer = warp == W;
   auto copy = [&](int i, int s) {
-    const int at         = (i < chunks ? i : i - chunks) * chunk;
+    const int at         = (i < chunks ? i : total - 1 - i) * chunk;
     const uint32_t bytes = (uint32_t)min(r.count - at, chunk) * 16u;
     mbar_arrive_expect_tx(&full[s], bytes);
     bulk_load_hint(smem + (size_t)s * slot_bytes, r.body + (size_t)(r.start + at) * 16, bytes, &full[s],
@@ -377,17 +377,18 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
   auto wait = [&]() {
     if (!dead && !mbar_wait_bounded(&full[slot], phase)) dead = true;
   };
-  auto leave = [&]() {  // the warp has read its part of the slot
-    if (!held) {
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[slot])) : "memory");
-    }
+  auto leave = [&](int s) {  // the warp has read its part of slot s
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[s])) : "memory");
+  };
+  auto next_slot = [&]() {
     if (++slot == N) {
       slot = 0;
       phase ^= 1;
     }
   };
-  for (int left = r.count; left > 0; left -= chunk) {
+  for (int i = 0; i < chunks; ++i) {
+    const int left = r.count - i * chunk;
     wait();
     const uint4* src = reinterpret_cast<const uint4*>(smem + (size_t)slot * slot_bytes) + tid;
     if (left >= chunk) {
@@ -401,9 +402,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
         walk<T, 1>(u, c, margin, k);
       }
     }
-    leave();
+    if (i < chunks - held) leave(slot);
+    next_slot();
   }
-  if (held) slot = 0;
   float p0, p1;
   unpair(add2(k.s0, k.s1), p0, p1);
   Sum t = warp_join({k.m, p0 + p1}, c);
@@ -480,18 +481,26 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
   if (GRAD) {
     // Pass 2: factor * 2^((x - M) c) / S everywhere, then the few columns that have a term of their own.
     const float coef = KIND == kDistill ? slope * inv_t : -slope * inv_t, q0 = coef / S;
-    for (int at = 0; at < r.count; at += chunk) {
-      const int left = r.count - at;
-      if (!held) wait();
-      const uint4* src = reinterpret_cast<const uint4*>(smem + (size_t)slot * slot_bytes) + tid;
+    int kept = (chunks - held) % N;  // slot of the first chunk that is still there
+    for (int i = 0; i < chunks; ++i) {
+      const int at = (i < held ? chunks - held + i : chunks - 1 - i) * chunk, left = r.count - at;
+      int s        = kept;
+      if (i < held) {
+        kept = kept + 1 == N ? 0 : kept + 1;
+      } else {
+        wait();
+        s = slot;
+        next_slot();
+      }
+      const uint4* src = reinterpret_cast<const uint4*>(smem + (size_t)s * slot_bytes) + tid;
       if (!live) {
         for (int j = tid; j < min(left, chunk); j += T32) put(at + j, make_uint4(0, 0, 0, 0));
-        leave();
+        leave(s);
       } else if (left >= chunk) {
         uint4 u[kUnroll];
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) u[j] = src[j * T32];
-        leave();
+        leave(s);
         common_part<T, kUnroll>(u, nM, c, q0);
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) put(at + tid + j * T32, u[j]);
@@ -501,7 +510,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
           common_part<T, 1>(u, nM, c, q0);
           put(at + j, u[0]);
         }
-        leave();
+        leave(s);
       }
     }
     if (edge >= 0) Io<T>::store1(gr + edge, live ? ex2((xe + nM) * c) * q0 : 0.0f);
