@@ -352,23 +352,54 @@ struct LossMatcher {
     s.args.push_back(Out(grad));
     for (int64_t v : {rows, cols, entries, wide, teacher}) s.args.push_back(I(v));
     s.args.push_back(weight < 0 ? F(0.0) : Constant(main.inputs[weight]));
-    s.args.push_back(F(Attr(main, "temperature")));
-    for (const char* key : {"clip_low", "clip_high", "kl_coef"}) s.args.push_back(F(kind == 1 ? Attr(main, key) : 0.0));
-    return ShapeRows(std::move(p), s, rows, cols * DTypeBytes(x.dtype), 12 * entries, grad != nullptr);
+    const double t = Attr(main, "temperature"), c = 1.4426950408889634 / t;  // exp(z / t) = 2^(c z)
+    for (double v : {1.0 / t, c, 24.0 / c}) s.args.push_back(F(v));
+    s.args.push_back(F(kind == 1 ? 1.0 - Attr(main, "clip_low") : 0.0));
+    s.args.push_back(F(kind == 1 ? 1.0 + Attr(main, "clip_high") : 0.0));
+    s.args.push_back(F(kind == 1 ? Attr(main, "kl_coef") : 0.0));
+    return ShapeRows(std::move(p), s, rows, cols * DTypeBytes(x.dtype), entries, grad != nullptr);
   }
 
   // Warps per CTA, CTAs per row and ring slots of the row kernels (row_loss.cu says what was measured).
   std::unique_ptr<CompiledGroup> ShapeRows(std::unique_ptr<CompiledGroup> p, LaunchStep s, int64_t rows, int64_t row_bytes,
-                                           int64_t kept_bytes, bool grad) {
-    const int64_t vecs = row_bytes / 16 + 1;
+                                           int64_t entries, bool grad) {
+    const int64_t vecs = row_bytes / 16;
     int64_t warps = 1, ctas = 1;
-    while (warps < 8 && warps * 256 < vecs) warps *= 2;
-    while (ctas < 8 && rows * ctas * 2 <= dev.sm_count && vecs > 32 * warps * ctas) ctas *= 2;
-    const int64_t slots = std::min<int64_t>(4, CeilDiv(vecs, 128 * warps));
-    if (rows * ctas > 2147483647) return Fail("more than 2^31 - 1 rows");
+    if (rows > 2147483647) return Fail("more than 2^31 - 1 rows");
+    // Short rows stay in registers: with the gradient up to 8 KiB (32768 x 4096 bf16 114 us, through a ring 128; 16 KiB 114
+    // against 113), without it up to 16 KiB (55 against 68).  Eight vectors per thread in one warp, or without the
+    // gradient; otherwise four, in more warps (114 us against 118).
+    const int64_t most_per = grad ? 4 : 8;
+    int64_t per            = 8;  // vectors per thread
+    if (vecs > 256) {
+      per = most_per;
+      while (warps < 4 && warps * 32 * per < vecs) warps *= 2;
+    }
+    if (warps * 32 * per >= vecs && entries <= 128) {
+      while (per > 2 && warps * 16 * per >= vecs) per /= 2;
+      const std::string name = std::string(s.kernel->name) + "_n" + std::to_string(per);
+      s.kernel = FindKernel(name);
+      if (!s.kernel) return Fail("kernel " + name + " is missing");
+      s.args.push_back(I(warps == 4 ? 2 : warps / 2));
+      s.dyn_smem = (size_t)(8 / warps * 16 * RoundUp(entries, 4));
+      s.block[0] = 256;
+      s.grid[0]  = (unsigned)CeilDiv(rows, 8 / warps);
+      p->steps.push_back(s);
+      return p;
+    }
+    // Few rows: smaller CTAs, and several of them for a row.  With the gradient 5.5 CTAs per SM in all (89 x 131072 bf16: 16 us
+    // with 8 CTAs per row, 24 with one), without it 2 (more of them wait for each other: 128 rows 11 us with 2, 13 with 4).
+    const int64_t most = dev.sm_count * (grad ? 11 : 4) / 2;
+    for (warps = 1; warps < 4 && warps * 256 < vecs;) warps *= 2;
+    if (rows * 2 <= most) {
+      while (ctas < 8 && rows * ctas * 2 <= most && vecs > 128 * warps * ctas) ctas *= 2;
+    } else {
+      if (vecs > 2048) warps = 8;  // (8192 x 16384 bf16: 93 us with 4 warps, 123 with 8; from 64 KiB on 8 are level or better)
+    }
+    const int64_t slots = std::min<int64_t>(4, CeilDiv(vecs + 1, 128 * warps));
     s.args.push_back(I(slots));
     s.cluster  = ctas > 1 ? (unsigned)ctas : 0;
-    s.dyn_smem = (size_t)(slots * (warps * 2048 + 16) + 8 + 8 * warps * ctas + kept_bytes);
+    s.dyn_smem = (size_t)(slots * (warps * 2048 + 16) + 8 + 8 * warps * ctas + 16 * RoundUp(entries, 4));
     s.block[0] = (unsigned)(32 * warps + 32);
     s.grid[0]  = (unsigned)(ctas * rows);
     p->steps.push_back(s);

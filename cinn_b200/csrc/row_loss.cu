@@ -43,7 +43,7 @@ CINN_B200_DEFINE_ASYNC_TIMEOUT_COUNTER(g_row_loss_wait_timeouts);
 namespace {
 
 enum Kind { kLogprob = 0, kPolicy = 1, kDistill = 2 };
-constexpr int kMaxWarps = 16;
+constexpr int kMaxWarps = 8;
 constexpr int kUnroll   = 4;   // 16-byte vectors per thread of a ring slot
 
 __device__ __forceinline__ long long load_index(const void* p, long long i, int wide) {
@@ -239,74 +239,262 @@ __device__ __forceinline__ Row row_at(const T* x, long long row, int cols, int r
   return r;
 }
 
+// The operands of a call, as the kernels get them.
+template <typename T>
+struct Call {
+  const T* x;
+  const void *ids, *a0;
+  const float *a1, *a2, *weight;
+  float *out_loss, *out_lp;
+  T* out_grad;
+  int cols, entries, wide, teacher;
+  float weight_value;
+  float inv_t, c, margin;  // 1 / temperature; the exponentials are 2^(c (x - reference)); by how much that moves at once
+  Policy policy;
+};
+#define ROW_LOSS_PARAMS                                                                                                  \
+  const T *__restrict__ x, const void *__restrict__ ids, const void *__restrict__ a0, const float *__restrict__ a1,       \
+      const float *__restrict__ a2, const float *__restrict__ weight, float *__restrict__ out_loss,                       \
+      float *__restrict__ out_lp, T *__restrict__ out_grad, long long rows, long long cols, long long entries,            \
+      long long wide, long long teacher, double weight_value, double inv_t, double c, double margin, double clip_low,     \
+      double clip_high, double kl_coef
+#define ROW_LOSS_CALL                                                                                                    \
+  {x, ids, a0, a1, a2, weight, out_loss, out_lp, out_grad, (int)cols, (int)entries, (int)wide, (int)teacher,              \
+   (float)weight_value, (float)inv_t, (float)c, (float)margin, {(float)clip_low, (float)clip_high, (float)kl_coef}}
+
+// What a row's scalar operands say.
+struct Head {
+  float w;
+  int a;      // the token's column, -1 outside
+  bool live;  // whether the row counts
+  bool need;  // whether it is read
+};
 template <typename T, int KIND, bool GRAD>
-__global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
-    k_row_loss(const T* __restrict__ x, const void* __restrict__ ids, const void* __restrict__ a0,
-               const float* __restrict__ a1, const float* __restrict__ a2, const float* __restrict__ weight,
-               float* __restrict__ out_loss, float* __restrict__ out_lp, T* __restrict__ out_grad, long long rows,
-               long long cols_ll, long long entries_ll, long long wide_ll, long long teacher_ll, double weight_value,
-               double temperature, double clip_low, double clip_high, double kl_coef, long long slots_ll) {
+__device__ __forceinline__ Head head_of(const Call<T>& o, long long row) {
+  Head h;
+  h.w                = o.weight ? __ldg(o.weight + row) : o.weight_value;
+  const long long id = KIND == kDistill ? 0 : load_index(o.ids, row, o.wide);
+  h.a                = id >= 0 && id < o.cols ? (int)id : -1;
+  h.live             = (GRAD || KIND != kLogprob) && h.w != 0.0f && h.a >= 0;
+  h.need             = h.live || (KIND != kDistill && o.out_lp && h.a >= 0);
+  return h;
+}
+struct PolicyOperands {
+  float old, ref, adv;
+};
+template <typename T, int KIND>
+__device__ __forceinline__ PolicyOperands policy_operands(const Call<T>& o, long long row) {
+  if (KIND != kPolicy) return {0.0f, 0.0f, 0.0f};
+  return {__ldg(static_cast<const float*>(o.a0) + row), o.policy.kl != 0.0f ? __ldg(o.a1 + row) : 0.0f, __ldg(o.a2 + row)};
+}
+
+// A row's teacher entries in shared memory, four arrays of `padded` values: their columns (-1: unused, -2: behind the last
+// one), their logits, the student's logits there, and (before the columns are stored) what all entries of a column have
+// together, over 2^(c (the largest)).
+struct Kept {
+  int* id;
+  float *t, *x, *mass;
+  int padded;
+};
+__device__ __forceinline__ Kept kept_at(void* p, int entries) {
+  const int n = (entries + 3) & ~3;
+  float* f    = static_cast<float*>(p);
+  return {static_cast<int*>(p), f + n, f + 2 * n, f + 3 * n, n};
+}
+template <typename T>
+__device__ __forceinline__ void keep_entries(const Call<T>& o, long long row, const Kept& k, int thread, int threads) {
+  for (int n = thread; n < k.padded; n += threads) {
+    if (n >= o.entries) {
+      k.id[n] = -2;
+      continue;
+    }
+    const long long i = load_index(o.ids, row * o.entries + n, o.wide);
+    const float t     = load_float(o.a0, row * o.entries + n, o.teacher);
+    const bool good   = i >= 0 && i < o.cols;
+    k.id[n]           = good ? (int)i : -1;
+    k.t[n]            = good ? t : -INFINITY;
+    k.x[n]            = good ? Io<T>::load1(o.x + row * o.cols + i) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void prefetch_entries(const Call<T>& o, long long row, int thread, int threads) {
+  const int wi = o.wide ? 8 : 4, wt = o.teacher ? 2 : 4;
+  const char* p0 = static_cast<const char*>(o.ids) + row * o.entries * wi;
+  const char* p1 = static_cast<const char*>(o.a0) + row * o.entries * wt;
+  for (int b = thread * 128; b < o.entries * wi; b += threads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p0 + b));
+  for (int b = thread * 128; b < o.entries * wt; b += threads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p1 + b));
+}
+
+// What follows from a row's sum: q_j = 2^(c (x_j + nm)) / S, the gradient's common part coef * q_j.
+struct Terms {
+  float nm, S, slope, coef, tmax, tsum;
+  bool live;
+};
+// Loss and log-probability are written by the lane for which `writes` holds (of the warp for which `sums` does, for the
+// distillation, whose sum over the entries a whole warp takes).
+template <typename T, int KIND>
+__device__ __forceinline__ Terms row_terms(const Call<T>& o, long long row, const Head& h, const Sum& t, float xa,
+                                           const PolicyOperands& po, const Kept& kept, bool writes, bool sums, int lane) {
+  Terms k        = {-finite_ref(t.m), t.s, h.w, 0.0f, -INFINITY, 0.0f, h.live};
+  const float lg = log2f(t.s);
+  auto logq      = [&](float v) { return ((v + k.nm) * o.c - lg) * 0.6931471805599453f; };
+  float loss     = 0.0f;
+  if (KIND != kDistill) {
+    const float lp = logq(xa);
+    if (KIND == kPolicy && h.live) {
+      policy_terms(lp, po.old, po.ref, po.adv, o.policy, &loss, &k.slope);
+      k.slope *= h.w;
+    }
+    if (writes) {
+      if (o.out_lp) o.out_lp[row] = lp;
+      if (o.out_loss) o.out_loss[row] = h.live ? h.w * loss : 0.0f;
+    }
+    k.coef = -k.slope * o.inv_t;
+    return k;
+  }
+  for (int n = lane; n < o.entries; n += 32) k.tmax = fmaxf(k.tmax, kept.t[n]);
+  k.tmax = warp_max(k.tmax);
+  k.live = k.tmax > -INFINITY;  // otherwise the teacher keeps nothing, and the row is out
+  for (int n = lane; n < o.entries && k.live; n += 32) k.tsum += ex2((kept.t[n] - k.tmax) * o.c);
+  k.tsum = warp_allreduce<SumOp>(k.tsum);
+  if (o.out_loss && sums) {
+    const float lt = log2f(k.tsum);
+    for (int n = lane; n < o.entries && k.live; n += 32) {
+      const float lp2 = (kept.t[n] - k.tmax) * o.c - lt, p = ex2(lp2);
+      if (p > 0.0f) loss += p * (lp2 * 0.6931471805599453f - logq(kept.x[n]));
+    }
+    loss = warp_allreduce<SumOp>(loss);
+    if (lane == 0) o.out_loss[row] = k.live ? h.w * loss : 0.0f;
+  }
+  k.coef = k.slope * o.inv_t;
+  return k;
+}
+// Every entry adds up its whole column, in the same order: entries of one column get the same value.  A column that no
+// other entry has (four are compared at a time) is its own sum.
+__device__ __forceinline__ void column_masses(const Kept& kept, int entries, const Terms& k, float c, int thread, int threads) {
+  for (int n = thread; n < entries; n += threads) {
+    const int id = kept.id[n];
+    int same     = 0;
+    for (int i = 0; i < kept.padded; i += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(kept.id + i);
+      same += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+    }
+    float mass = ex2((kept.t[n] - k.tmax) * c);
+    if (same > 1 && id >= 0) {
+      mass = 0.0f;
+      for (int i = 0; i < entries; ++i)
+        if (kept.id[i] == id) mass += ex2((kept.t[i] - k.tmax) * c);
+    }
+    kept.mass[n] = mass;
+  }
+}
+// The columns that have a term of their own, stored again by the warp that stored their vectors (`mine`).
+template <typename T, int KIND, class Mine>
+__device__ __forceinline__ void special_columns(const Call<T>& o, T* gr, const Terms& k, const Head& h, float xa,
+                                                const Kept& kept, int lane, Mine mine) {
+  if (KIND != kDistill) {
+    if (k.live && lane == 0 && mine(h.a)) Io<T>::store1(gr + h.a, k.slope * o.inv_t * (1.0f - __fdividef(ex2((xa + k.nm) * o.c), k.S)));
+  } else if (k.live) {
+    const float it = 1.0f / k.tsum;
+    for (int n = lane; n < o.entries; n += 32) {
+      const int id = kept.id[n];
+      if (id >= 0 && mine(id)) Io<T>::store1(gr + id, k.coef * (__fdividef(ex2((kept.x[n] + k.nm) * o.c), k.S) - kept.mass[n] * it));
+    }
+  }
+}
+// A vector of the gradient at `p`, which may not be aligned as the logits are.
+template <typename T>
+__device__ __forceinline__ void put(char* p, uint4 u) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    st_stream16(p, u);
+    return;
+  }
+  const uint32_t t[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 16 / (int)sizeof(T); ++j) {
+    T one;
+    if constexpr (sizeof(T) == 4) one = __uint_as_float(t[j]);
+    else reinterpret_cast<unsigned short&>(one) = (unsigned short)(t[j / 2] >> (16 * (j & 1)));
+    reinterpret_cast<T*>(p)[j] = one;
+  }
+}
+// The element in front of or behind a row's vectors that a lane of its first warp holds, -1 if none.
+__device__ __forceinline__ int edge_of(const Row& r, int cols, bool first_warp, int lane) {
+  if (!first_warp) return -1;
+  return lane < r.head ? lane : lane >= 8 && lane - 8 < r.tail ? cols - r.tail + lane - 8 : -1;
+}
+__device__ __forceinline__ Walk start_walk(float xe, float c) {
+  Walk k;
+  k.m  = xe == xe ? xe : -INFINITY;
+  k.nm = -finite_ref(k.m);
+  k.s0 = pair(ex2((xe + k.nm) * c), 0.0f);
+  k.s1 = pair(0.0f, 0.0f);
+  return k;
+}
+__device__ __forceinline__ Sum end_walk(const Walk& k, float c) {
+  float lo, hi;
+  unpair(add2(k.s0, k.s1), lo, hi);
+  return warp_join({k.m, lo + hi}, c);
+}
+__device__ __forceinline__ Sum join_all(const float2* meet, int n, int lane, float c) {
+  Sum u = {-INFINITY, 0.0f};
+  for (int i = lane; i < n; i += 32) {
+    const float2 v = meet[i];
+    const float hi = fmaxf(u.m, v.x), hf = finite_ref(hi);
+    u.s = u.s * ex2((u.m - hf) * c) + v.y * ex2((v.x - hf) * c);
+    u.m = hi;
+  }
+  return warp_join(u, c);
+}
+// The barrier of one row's threads (numbers that the compiler knows: a number at run time reserves all sixteen).
+__device__ __forceinline__ void barrier_of(int group, int threads) {
+  switch (group) {
+    case 0: asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); break;
+    case 1: asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory"); break;
+    case 2: asm volatile("bar.sync 3, %0;" ::"r"(threads) : "memory"); break;
+    default: asm volatile("bar.sync 4, %0;" ::"r"(threads) : "memory"); break;
+  }
+}
+
+template <typename T, int KIND, bool GRAD>
+__global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PARAMS, long long slots_ll) {
   grid_dependency_sync();
   constexpr int V = 16 / sizeof(T);
   extern __shared__ __align__(128) unsigned char smem[];
-  const int cols = (int)cols_ll, entries = (int)entries_ll, wide = (int)wide_ll, teacher = (int)teacher_ll;
+  const Call<T> o = ROW_LOSS_CALL;
   const int N = (int)slots_ll, W = (blockDim.x >> 5) - 1, T32 = W * 32, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int C, rank;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int G = C * W, g = rank * W + warp, slot_bytes = T32 * kUnroll * 16;
   const long long row = blockIdx.x / C;
-  uint64_t* full  = reinterpret_cast<uint64_t*>(smem + (size_t)N * slot_bytes);
+  const Kept kept = kept_at(smem + (size_t)N * slot_bytes, o.entries);
+  uint64_t* full  = reinterpret_cast<uint64_t*>(kept.mass + kept.padded);
   uint64_t* empty = full + N;
-  uint64_t* met   = empty + N;                             // completes when the pairs of all G warps are here
-  float2* meet    = reinterpret_cast<float2*>(met + 1);    // [G]
-  int* kept_id    = reinterpret_cast<int*>(meet + G);      // [entries], the distillation's
-  float* kept_t   = reinterpret_cast<float*>(kept_id + entries);
-  float* kept_x   = kept_t + entries;
-  const float c   = (float)(1.4426950408889634 / temperature);
+  uint64_t* met   = empty + N;                           // completes when the pairs of all G warps are here
+  float2* meet    = reinterpret_cast<float2*>(met + 1);  // [G]
   const T* xr     = x + row * cols;
-
-  const float w  = weight ? __ldg(weight + row) : (float)weight_value;
-  long long id   = KIND == kDistill ? 0 : load_index(ids, row, wide);
-  const int a    = id >= 0 && id < cols ? (int)id : -1;
-  bool live      = (GRAD || KIND != kLogprob) && w != 0.0f && a >= 0;  // whether the row counts
-  const bool need = live || (KIND != kDistill && out_lp && a >= 0);    // whether it is read
-  const Row r    = row_at(x, row, cols, rank, C);
-  // The element in front of or behind the vectors that this lane holds, if any (first warp of the row).
-  const int edge = g == 0 && lane < r.head ? lane : g == 0 && lane >= 8 && lane - 8 < r.tail ? cols - r.tail + lane - 8 : -1;
-
-  T* gr      = GRAD ? out_grad + row * cols : nullptr;
-  char* body = GRAD ? reinterpret_cast<char*>(gr + r.head) + (size_t)r.start * 16 : nullptr;
-  auto put   = [&](int v, uint4 u) {  // a vector of the gradient
-    if ((reinterpret_cast<uintptr_t>(body) & 15) == 0) {
-      st_stream16(body + (size_t)v * 16, u);
-    } else {  // the gradient is not aligned as the logits are
-      const uint32_t t[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        T one;
-        if constexpr (sizeof(T) == 4) one = __uint_as_float(t[j]);
-        else reinterpret_cast<unsigned short&>(one) = (unsigned short)(t[j / 2] >> (16 * (j & 1)));
-        reinterpret_cast<T*>(body)[v * V + j] = one;
-      }
-    }
-  };
-  if (!need) {  // the same for every warp of the row: no barrier is left waiting
+  const Head h    = head_of<T, KIND, GRAD>(o, row);
+  const Row r     = row_at(x, row, o.cols, rank, C);
+  const int edge  = edge_of(r, o.cols, g == 0, lane);
+  T* gr           = GRAD ? out_grad + row * cols : nullptr;
+  char* body      = GRAD ? reinterpret_cast<char*>(gr + r.head) + (size_t)r.start * 16 : nullptr;
+  if (!h.need) {  // the same for every warp of the row: no barrier is left waiting
     if (g == 0 && lane == 0) {
       if (out_loss) out_loss[row] = 0.0f;
       if (out_lp) out_lp[row] = 0.0f;
     }
     if (GRAD) {
-      for (int v = tid; v < r.count; v += blockDim.x) put(v, make_uint4(0, 0, 0, 0));
+      for (int v = tid; v < r.count; v += blockDim.x) put<T>(body + (size_t)v * 16, make_uint4(0, 0, 0, 0));
       if (edge >= 0) Io<T>::store1(gr + edge, 0.0f);
     }
     return;
   }
 
-  const int chunk  = T32 * kUnroll;                               // vectors of a slot
+  const int chunk  = T32 * kUnroll;                          // vectors of a slot
   const int chunks = (r.count + chunk - 1) / chunk;
-  const int held   = GRAD ? min(chunks, N) : 0;                   // pass 2 finds the last ones still in the ring
-  const int total  = GRAD ? 2 * chunks - held : chunks;           // and has the others fetched again, last one first
+  const int held   = GRAD ? min(chunks, N) : 0;              // pass 2 finds the last ones still in the ring
+  const int total  = GRAD ? 2 * chunks - held : chunks;      // and has the others fetched again, last one first
   const bool producer = warp == W;
   auto copy = [&](int i, int s) {
     const int at         = (i < chunks ? i : total - 1 - i) * chunk;
@@ -349,28 +537,14 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
     if (C > 1) cluster_barrier();
     return;
   }
-  float xe = -INFINITY, xa = 0.0f, old = 0.0f, ref = 0.0f, adv = 0.0f;
+  float xe = -INFINITY, xa = 0.0f;
   if (edge >= 0) xe = Io<T>::load1(xr + edge);
-  if (KIND != kDistill) xa = Io<T>::load1(xr + a);
-  if (KIND == kPolicy) {
-    old = __ldg(static_cast<const float*>(a0) + row);
-    ref = kl_coef != 0.0 ? __ldg(a1 + row) : 0.0f;
-    adv = __ldg(a2 + row);
-  }
-  if (KIND == kDistill) {  // the teacher's entries into L2; they are wanted after pass 1
-    const char* p0 = static_cast<const char*>(ids) + row * entries * (wide ? 8 : 4);
-    const char* p1 = static_cast<const char*>(a0) + row * entries * (teacher ? 2 : 4);
-    for (int b = tid * 128; b < entries * (wide ? 8 : 4); b += T32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p0 + b));
-    for (int b = tid * 128; b < entries * (teacher ? 2 : 4); b += T32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p1 + b));
-  }
+  if (KIND != kDistill) xa = Io<T>::load1(xr + h.a);
+  const PolicyOperands po = policy_operands<T, KIND>(o, row);
+  if (KIND == kDistill) prefetch_entries(o, row, tid, T32);  // they are wanted after pass 1
 
   // Pass 1.
-  Walk k;
-  k.m  = xe == xe ? xe : -INFINITY;
-  k.nm = -finite_ref(k.m);
-  k.s0 = pair(ex2((xe + k.nm) * c), 0.0f);
-  k.s1 = pair(0.0f, 0.0f);
-  const float margin = 24.0f / c;
+  Walk k   = start_walk(xe, o.c);
   int slot = 0;  // next slot to read, and the parity of its phase
   uint32_t phase = 0;
   bool dead = false;
@@ -395,33 +569,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
       uint4 u[kUnroll];
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j) u[j] = src[j * T32];
-      walk<T, kUnroll>(u, c, margin, k);
+      walk<T, kUnroll>(u, o.c, o.margin, k);
     } else {
       for (int j = tid; j < left; j += T32) {
         const uint4 u[1] = {src[j - tid]};
-        walk<T, 1>(u, c, margin, k);
+        walk<T, 1>(u, o.c, o.margin, k);
       }
     }
     if (i < chunks - held) leave(slot);
     next_slot();
   }
-  float p0, p1;
-  unpair(add2(k.s0, k.s1), p0, p1);
-  Sum t = warp_join({k.m, p0 + p1}, c);
-  if (KIND == kDistill) {  // the entries and the student's logits at them, for every warp of this CTA
-    for (int n = tid; n < entries; n += T32) {
-      const long long i = load_index(ids, row * entries + n, wide);
-      const float tn    = load_float(a0, row * entries + n, teacher);
-      const bool good   = i >= 0 && i < cols;
-      kept_id[n]        = good ? (int)i : -1;
-      kept_t[n]         = good ? tn : -INFINITY;
-      kept_x[n]         = good ? Io<T>::load1(xr + i) : 0.0f;
-    }
-  }
+  Sum t = end_walk(k, o.c);
+  if (KIND == kDistill) keep_entries(o, row, kept, tid, T32);  // for every warp of this CTA
   if (G > 1) {
     if (C == 1) {
       if (lane == 0) meet[warp] = make_float2(t.m, t.s);
-      asm volatile("bar.sync 1, %0;" ::"r"(T32) : "memory");
+      barrier_of(0, T32);
     } else {
       if (lane < C) {
         uint32_t there, bar;
@@ -431,130 +594,156 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 1)
                      : "memory");
       }
       __syncwarp();
-      if (KIND == kDistill) asm volatile("bar.sync 1, %0;" ::"r"(T32) : "memory");  // the entries above
+      if (KIND == kDistill) barrier_of(0, T32);  // the entries above
       if (!dead && !mbar_wait_bounded(met, 0)) dead = true;
     }
-    Sum u = {-INFINITY, 0.0f};
-    for (int n = lane; n < G; n += 32) {
-      const float2 o = meet[n];
-      const float hi = fmaxf(u.m, o.x), hf = finite_ref(hi);
-      u.s = u.s * ex2((u.m - hf) * c) + o.y * ex2((o.x - hf) * c);
-      u.m = hi;
-    }
-    t = warp_join(u, c);
+    t = join_all(meet, G, lane, o.c);
   } else {
     __syncwarp();
   }
-  const float nM = -finite_ref(t.m), S = t.s, lg = log2f(S), inv_t = (float)(1.0 / temperature);
-  auto logq = [&](float v) { return ((v + nM) * c - lg) * 0.6931471805599453f; };
-
-  float slope = w, loss = 0.0f;  // slope: d loss / d lp, or the factor of the softmax for the distillation
-  float tmax = -INFINITY, tsum = 0.0f;
-  if (KIND != kDistill) {
-    const float lp = logq(xa);
-    if (KIND == kPolicy && live) {
-      const Policy pol = {(float)(1.0 - clip_low), (float)(1.0 + clip_high), (float)kl_coef};
-      policy_terms(lp, old, ref, adv, pol, &loss, &slope);
-      slope *= w;
-    }
-    if (g == 0 && lane == 0) {
-      if (out_lp) out_lp[row] = lp;
-      if (out_loss) out_loss[row] = live ? w * loss : 0.0f;
-    }
-  } else {
-    for (int n = lane; n < entries; n += 32) tmax = fmaxf(tmax, kept_t[n]);
-    tmax = warp_max(tmax);
-    live = tmax > -INFINITY;  // otherwise the teacher keeps nothing, and the row is out
-    for (int n = lane; n < entries && live; n += 32) tsum += ex2((kept_t[n] - tmax) * c);
-    tsum = warp_allreduce<SumOp>(tsum);
-    if (out_loss && g == G - 1) {  // one warp of the row
-      const float lt = log2f(tsum);
-      for (int n = lane; n < entries && live; n += 32) {
-        const float lp2 = (kept_t[n] - tmax) * c - lt, p = ex2(lp2);
-        if (p > 0.0f) loss += p * (lp2 * 0.6931471805599453f - logq(kept_x[n]));
-      }
-      loss = warp_allreduce<SumOp>(loss);
-      if (lane == 0) out_loss[row] = live ? w * loss : 0.0f;
-    }
-  }
+  const Terms m = row_terms<T, KIND>(o, row, h, t, xa, po, kept, g == 0 && lane == 0, g == G - 1, lane);
 
   if (GRAD) {
-    // Pass 2: factor * 2^((x - M) c) / S everywhere, then the few columns that have a term of their own.
-    const float coef = KIND == kDistill ? slope * inv_t : -slope * inv_t, q0 = coef / S;
-    int kept = (chunks - held) % N;  // slot of the first chunk that is still there
+    if (KIND == kDistill) column_masses(kept, o.entries, m, o.c, tid, T32);
+    // Pass 2: coef * q_j everywhere, then the few columns that have a term of their own.
+    const float q0 = __fdividef(m.coef, m.S);
+    int there      = (chunks - held) % N;  // slot of the first chunk that is still there
     for (int i = 0; i < chunks; ++i) {
       const int at = (i < held ? chunks - held + i : chunks - 1 - i) * chunk, left = r.count - at;
-      int s        = kept;
+      int s        = there;
       if (i < held) {
-        kept = kept + 1 == N ? 0 : kept + 1;
+        there = there + 1 == N ? 0 : there + 1;
       } else {
         wait();
         s = slot;
         next_slot();
       }
       const uint4* src = reinterpret_cast<const uint4*>(smem + (size_t)s * slot_bytes) + tid;
-      if (!live) {
-        for (int j = tid; j < min(left, chunk); j += T32) put(at + j, make_uint4(0, 0, 0, 0));
+      char* dst        = body + (size_t)(at + tid) * 16;
+      if (!m.live) {
+        for (int j = tid; j < min(left, chunk); j += T32) put<T>(dst + (size_t)(j - tid) * 16, make_uint4(0, 0, 0, 0));
         leave(s);
       } else if (left >= chunk) {
         uint4 u[kUnroll];
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j) u[j] = src[j * T32];
         leave(s);
-        common_part<T, kUnroll>(u, nM, c, q0);
+        common_part<T, kUnroll>(u, m.nm, o.c, q0);
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) put(at + tid + j * T32, u[j]);
+        for (int j = 0; j < kUnroll; ++j) put<T>(dst + (size_t)j * T32 * 16, u[j]);
       } else {
         for (int j = tid; j < left; j += T32) {
           uint4 u[1] = {src[j - tid]};
-          common_part<T, 1>(u, nM, c, q0);
-          put(at + j, u[0]);
+          common_part<T, 1>(u, m.nm, o.c, q0);
+          put<T>(dst + (size_t)(j - tid) * 16, u[0]);
         }
         leave(s);
       }
     }
-    if (edge >= 0) Io<T>::store1(gr + edge, live ? ex2((xe + nM) * c) * q0 : 0.0f);
-    // Columns are stored again by the warp that stored them above (ordered by the warp barrier).
-    __syncwarp();
-    auto mine = [&](int i) {
+    if (edge >= 0) Io<T>::store1(gr + edge, m.live ? ex2((xe + m.nm) * o.c) * q0 : 0.0f);
+    __syncwarp();  // the vectors before what is stored over them
+    if (KIND == kDistill) barrier_of(0, T32);  // the masses
+    special_columns<T, KIND>(o, gr, m, h, xa, kept, lane, [&](int i) {
       const int e = i - r.head;
       if (e < 0 || e >= r.nvec * V) return g == 0;
       const int at = e / V - r.start;
-      return at >= 0 && at < r.count && (at % T32) / 32 == warp;
-    };
-    if (KIND != kDistill) {
-      if (live && lane == 0 && mine(a)) Io<T>::store1(gr + a, slope * inv_t * (1.0f - ex2((xa + nM) * c) / S));
-    } else if (live) {
-      const float it = 1.0f / tsum;
-      for (int n0 = 0; n0 < entries; n0 += 32) {
-        const int i   = n0 + lane < entries ? kept_id[n0 + lane] : -1;
-        unsigned todo = __ballot_sync(0xffffffffu, i >= 0 && mine(i));
-        while (todo) {  // one column at a time: the warp adds up all of its entries
-          const int n   = __ffs(todo) - 1;
-          const int col = __shfl_sync(0xffffffffu, i, n);
-          todo &= todo - 1;
-          float p = 0.0f;
-          for (int n2 = lane; n2 < entries; n2 += 32)
-            if (kept_id[n2] == col) p += ex2((kept_t[n2] - tmax) * c);
-          p = warp_allreduce<SumOp>(p) * it;
-          if (lane == 0) Io<T>::store1(gr + col, coef * (ex2((kept_x[n0 + n] + nM) * c) / S - p));
-        }
-      }
-    }
+      return at >= 0 && at < r.count && (at & (T32 - 1)) / 32 == warp;
+    });
   }
   if (__any_sync(0xffffffffu, dead) && lane == 0) atomicAdd(&g_row_loss_wait_timeouts, 1u);
   if (C > 1) cluster_barrier();  // no CTA leaves while another may still write to its shared memory
 }
 
+// Rows of at most 16 KiB, in registers: W = 2^shift warps per row (1, 2 or 4), 8 / W rows per CTA, up to NV vectors per thread, all
+// of them loaded at once.  A row's warps meet at a barrier of their own.
+template <typename T, int KIND, bool GRAD, int NV>
+__global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOSS_PARAMS, long long shift_ll) {
+  grid_dependency_sync();
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float2 meet[8];
+  const Call<T> o = ROW_LOSS_CALL;
+  const int W = 1 << (int)shift_ll, T32 = 32 * W, group = threadIdx.x >> (5 + (int)shift_ll), tid = threadIdx.x - group * T32, lane = tid & 31, warp = tid >> 5;
+  const long long row = (long long)blockIdx.x * (8 >> (int)shift_ll) + group;
+  if (row >= rows) return;
+  const Kept kept = kept_at(smem + group * ((o.entries + 3) & ~3) * 16, o.entries);
+  const T* xr     = x + row * cols;
+  const Head h    = head_of<T, KIND, GRAD>(o, row);
+  const Row r     = row_at(x, row, o.cols, 0, 1);
+  const int edge  = edge_of(r, o.cols, warp == 0, lane);
+  T* gr           = GRAD ? out_grad + row * cols : nullptr;
+  char* body      = GRAD ? reinterpret_cast<char*>(gr + r.head) : nullptr;
+  if (!h.need) {
+    if (tid == 0) {
+      if (out_loss) out_loss[row] = 0.0f;
+      if (out_lp) out_lp[row] = 0.0f;
+    }
+    if (GRAD) {
+      for (int v = tid; v < r.nvec; v += T32) put<T>(body + (size_t)v * 16, make_uint4(0, 0, 0, 0));
+      if (edge >= 0) Io<T>::store1(gr + edge, 0.0f);
+    }
+    return;
+  }
+  uint4 u[NV];
+  const uint4* src = reinterpret_cast<const uint4*>(r.body) + tid;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) u[j] = tid + j * T32 < r.nvec ? ld_stream16(src + j * T32) : minus_infinity<T>();
+  float xe = -INFINITY, xa = 0.0f;
+  if (edge >= 0) xe = Io<T>::load1(xr + edge);
+  if (KIND != kDistill) xa = Io<T>::load1(xr + h.a);
+  const PolicyOperands po = policy_operands<T, KIND>(o, row);
+  if (KIND == kDistill) keep_entries(o, row, kept, tid, T32);
+  Walk k = start_walk(xe, o.c);
+  if constexpr (NV == 8) {
+    walk<T, 4>(reinterpret_cast<const uint4(&)[4]>(u[0]), o.c, o.margin, k);
+    walk<T, 4>(reinterpret_cast<const uint4(&)[4]>(u[4]), o.c, o.margin, k);
+  } else {
+    walk<T, NV>(u, o.c, o.margin, k);
+  }
+  Sum t = end_walk(k, o.c);
+  if (W > 1) {
+    if (lane == 0) meet[group * W + warp] = make_float2(t.m, t.s);
+    barrier_of(group, T32);
+    t = join_all(meet + group * W, W, lane, o.c);
+  } else {
+    __syncwarp();
+  }
+  const Terms m = row_terms<T, KIND>(o, row, h, t, xa, po, kept, tid == 0, warp == W - 1, lane);
+  if (!GRAD) return;
+  if (KIND == kDistill) column_masses(kept, o.entries, m, o.c, tid, T32);
+  const float q0 = __fdividef(m.coef, m.S);
+  if (m.live) {
+    common_part<T, NV>(u, m.nm, o.c, q0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) u[j] = make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (tid + j * T32 < r.nvec) put<T>(body + (size_t)(tid + j * T32) * 16, u[j]);
+  if (edge >= 0) Io<T>::store1(gr + edge, m.live ? ex2((xe + m.nm) * o.c) * q0 : 0.0f);
+  __syncwarp();  // the vectors before what is stored over them
+  if (KIND == kDistill && W > 1) barrier_of(group, T32);  // the masses
+  special_columns<T, KIND>(o, gr, m, h, xa, kept, lane, [&](int i) {
+    const int e = i - r.head;
+    return e < 0 || e >= r.nvec * V ? warp == 0 : ((e / V) & (T32 - 1)) / 32 == warp;
+  });
+}
+
 }  // namespace
 
-#define REG_ROW_LOSS(KNAME, KIND, TNAME, T)                                                                          \
-  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME "_" TNAME, 20, kMaxWarps * 32 + 32, k_row_loss<T, KIND, false>);         \
-  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME "_grad_" TNAME, 20, kMaxWarps * 32 + 32, k_row_loss<T, KIND, true>)
-#define REG_ROW_LOSS_KINDS(TNAME, T)             \
-  REG_ROW_LOSS("logprob", kLogprob, TNAME, T);   \
-  REG_ROW_LOSS("policy", kPolicy, TNAME, T);     \
-  REG_ROW_LOSS("distill", kDistill, TNAME, T)
+#define REG_ROW_LOSS(KNAME, KIND, GNAME, GRAD, TNAME, T)                                                                      \
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME, 22, kMaxWarps * 32 + 32, k_row_loss<T, KIND, GRAD>);         \
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n2", 22, 256, k_row_loss_short<T, KIND, GRAD, 2>);          \
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n4", 22, 256, k_row_loss_short<T, KIND, GRAD, 4>);          \
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n8", 22, 256, k_row_loss_short<T, KIND, GRAD, 8>)
+#define REG_ROW_LOSS_KINDS(TNAME, T)                           \
+  REG_ROW_LOSS("logprob", kLogprob, "", false, TNAME, T);      \
+  REG_ROW_LOSS("logprob", kLogprob, "_grad", true, TNAME, T);  \
+  REG_ROW_LOSS("policy", kPolicy, "", false, TNAME, T);        \
+  REG_ROW_LOSS("policy", kPolicy, "_grad", true, TNAME, T);    \
+  REG_ROW_LOSS("distill", kDistill, "", false, TNAME, T);      \
+  REG_ROW_LOSS("distill", kDistill, "_grad", true, TNAME, T)
 REG_ROW_LOSS_KINDS("f32", float);
 REG_ROW_LOSS_KINDS("f16", __half);
 REG_ROW_LOSS_KINDS("bf16", __nv_bfloat16);
