@@ -214,11 +214,10 @@ int NetBuilder::AddOp(const std::string& op, const std::vector<int>& inputs,
     return AddOp("reshape", inputs, {{"shape", JoinInts(shape)}}, err);
   }
   if (op == "balance_loss") {
-    // Column sums of the routing probabilities, then one number from them: two instructions, the first of which shares
-    // its pass over the logits with balance_loss_grad.
+    // Sums over parts of the tokens, which share their pass over the logits with balance_loss_grad, then their sum.
     if (!need(3)) return fail("takes 3 inputs (logits, counts, weight)");
-    const int load = AddOp("expert_load", {inputs[0], inputs[2]}, {}, err);
-    return load < 0 ? -1 : AddOp("balance_fold", {load, inputs[1]}, {}, err);
+    const int part = AddOp("balance_part", inputs, {}, err);
+    return part < 0 ? -1 : AddOp("reduce_sum", {part}, {}, err);
   }
   Variable out;
   if (IsLossOp(op)) {

@@ -47,8 +47,7 @@ const Spec kSpecs[] = {
     {"distill_loss", 4, 3, "(logits, teacher_logits, teacher_index, weight)"},
     {"distill_loss_grad", 4, 3, "(logits, teacher_logits, teacher_index, weight)"},
     {"expert_counts", 2, 1, "(index, weight)"},
-    {"expert_load", 2, 1, "(logits, weight)"},
-    {"balance_fold", 2, -1, "(load, counts)"},
+    {"balance_part", 3, 2, "(logits, counts, weight)"},
     {"balance_loss_grad", 3, 2, "(logits, counts, weight)"},
 };
 const Spec* FindSpec(const std::string& op) {
@@ -62,9 +61,9 @@ bool EndsWith(const std::string& s, const char* tail) {
   return s.size() >= t.size() && s.compare(s.size() - t.size(), t.size(), t) == 0;
 }
 
-// In how many slices of the tokens expert_load sums a column: a slice per CTA of its kernel, at least 64 tokens
-// each, two CTAs per SM of a B200 at most.  It is the extent of the op's result, so it depends on the shape alone.
-int64_t LoadSlices(int64_t rows) { return std::min<int64_t>(CeilDiv(rows, 64), 296); }
+// In how many sums over tokens balance_part leaves the loss: one per CTA of its kernel, at least 64 tokens each, two CTAs
+// per SM of a B200 at most.  It is the extent of the op's result, so it depends on the shape alone.
+int64_t BalanceParts(int64_t rows) { return std::min<int64_t>(CeilDiv(rows, 64), 296); }
 
 }  // namespace
 
@@ -120,28 +119,18 @@ bool InferLossOp(const std::string& op, const std::vector<TensorDesc>& in, std::
     if (n > 2147483647) return fail("more than 2^31 - 1 choices: the counts are int32");
     return true;
   }
-  if (op == "balance_fold") {
-    if (in[0].dtype != DType::kFloat32 || in[0].shape.size() != 2) return fail("load must be float32 [slices, experts]");
-    if (in[1].dtype != DType::kInt32 || in[1].shape != std::vector<int64_t>{in[0].shape[1]})
-      return fail("counts must be int32 [experts]");
-    if (in[0].shape[1] > kMaxExperts) return fail("at most " + std::to_string(kMaxExperts) + " experts");
-    out->dtype = DType::kFloat32;
-    out->shape = {1};
-    return true;
-  }
   const TensorDesc& x = in[0];
   if (!IsLogits(x.dtype)) return fail("logits must be float32, float16 or bfloat16");
   if (x.shape.size() < 2) return fail("logits must be [rows..., columns]");
   const int64_t cols = x.shape.back(), rows = x.numel() / cols;
   const std::vector<int64_t> row_shape(x.shape.begin(), x.shape.end() - 1);
-  if (op == "expert_load" || op == "balance_loss_grad") {
+  if (op == "balance_part" || op == "balance_loss_grad") {
     if (cols > kMaxExperts) return fail("at most " + std::to_string(kMaxExperts) + " experts");
+    if (in[1].dtype != DType::kInt32 || in[1].shape != std::vector<int64_t>{cols}) return fail("counts must be int32 [experts]");
+    if (!per_row(in[2], x, "weight", DType::kFloat32)) return false;
     const bool grad = op == "balance_loss_grad";
-    if (!per_row(in[grad ? 2 : 1], x, "weight", DType::kFloat32)) return false;
-    if (grad && (in[1].dtype != DType::kInt32 || in[1].shape != std::vector<int64_t>{cols}))
-      return fail("counts must be int32 [experts]");
     out->dtype = grad ? x.dtype : DType::kFloat32;
-    out->shape = grad ? x.shape : std::vector<int64_t>{LoadSlices(rows), cols};
+    out->shape = grad ? x.shape : std::vector<int64_t>{BalanceParts(rows)};
     return true;
   }
   if (!number("temperature", 1.0, positive, "a number from 1e-4 to 1e4")) return false;
@@ -302,11 +291,7 @@ struct LossMatcher {
       if (ops.size() != 1) return Fail("expert_counts has a kernel of its own");
       return PlanCounts(*op);
     }
-    if (const OpDesc* op = get("balance_fold")) {
-      if (ops.size() != 1) return Fail("balance_fold has a kernel of its own");
-      return PlanFold(*op);
-    }
-    if (only({"expert_load", "balance_loss_grad"})) return PlanRouter(get("expert_load"), get("balance_loss_grad"));
+    if (only({"balance_part", "balance_loss_grad"})) return PlanRouter(get("balance_part"), get("balance_loss_grad"));
     if (only({"distill_loss", "distill_loss_grad"})) return PlanRows(2, get("distill_loss"), get("distill_loss_grad"), nullptr);
     if (only({"policy_loss", "policy_loss_grad", "token_logprob"}) && (get("policy_loss") || get("policy_loss_grad")))
       return PlanRows(1, get("policy_loss"), get("policy_loss_grad"), get("token_logprob"));
@@ -406,43 +391,44 @@ struct LossMatcher {
     return p;
   }
 
-  std::unique_ptr<CompiledGroup> PlanRouter(const OpDesc* load, const OpDesc* grad) {
-    if (load && grad && (load->inputs[0] != grad->inputs[0] || load->inputs[1] != grad->inputs[2]))
-      return Fail("the load and the gradient differ in an operand");
-    const OpDesc& main  = grad ? *grad : *load;
+  std::unique_ptr<CompiledGroup> PlanRouter(const OpDesc* part, const OpDesc* grad) {
+    if (part && grad && part->inputs != grad->inputs) return Fail("the loss and its gradient differ in an operand");
+    const OpDesc& main  = grad ? *grad : *part;
     const TensorDesc& x = Input(main.inputs[0]);
     const int64_t cols = x.shape.back(), rows = x.numel() / cols;
     auto p = NewPlan("router_loss");
     // Vector loads need rows that start on 16-byte boundaries; other rows, and buffers that do not, go by elements.
     const int64_t vec = 16 / DTypeBytes(x.dtype);
-    if (!RouterStep(load, grad, x, rows, cols, 1, cols % vec == 0 ? &p->steps_unaligned : &p->steps)) return nullptr;
+    if (!RouterStep(part, grad, rows, cols, 1, cols % vec == 0 ? &p->steps_unaligned : &p->steps)) return nullptr;
     if (cols % vec == 0) {
-      if (!RouterStep(load, grad, x, rows, cols, vec, &p->steps)) return nullptr;
+      if (!RouterStep(part, grad, rows, cols, vec, &p->steps)) return nullptr;
       p->aligned_inputs = {In(main.inputs[0]).index};
       if (grad) p->aligned_outputs = {Out(grad).index};
     }
     return p;
   }
-  bool RouterStep(const OpDesc* load, const OpDesc* grad, const TensorDesc& x, int64_t rows, int64_t cols, int64_t vec,
-                  std::vector<LaunchStep>* steps) {
-    const OpDesc& main = grad ? *grad : *load;
-    const int64_t vecs = cols / vec;
-    int64_t lanes = 1, per = 1;  // lanes of a token's row, vectors per lane
-    while (lanes < 32 && lanes < vecs) lanes *= 2;
+  bool RouterStep(const OpDesc* part, const OpDesc* grad, int64_t rows, int64_t cols, int64_t vec, std::vector<LaunchStep>* steps) {
+    const OpDesc& main  = grad ? *grad : *part;
+    const TensorDesc& x = Input(main.inputs[0]);
+    const int64_t vecs  = cols / vec;
+    // A token's row over as many lanes as give each about eight elements: the reductions over the lanes, 15 shuffles over
+    // 32 of them, then weigh little (65536 x 256 fp32: 32 us in all; with sixteen elements 34, fewer warps fit an SM).
+    int64_t lanes = 1, per = 1;
+    while (per < 8 / vec && per < vecs) per *= 2;
+    while (lanes < 32 && lanes * per < vecs) lanes *= 2;
     while (lanes * per < vecs) per *= 2;
     LaunchStep s;
     const std::string name = std::string("router_loss_") + ShortName(x.dtype) + (vec > 1 ? "_v" : "_s") + "_n" + std::to_string(per);
     s.kernel = FindKernel(name);
     if (!s.kernel) return Fail("kernel " + name + " is missing") != nullptr;
-    s.args = {In(main.inputs[0]), In(main.inputs.back()), grad ? In(grad->inputs[1]) : ArgSpec(), Out(load), Out(grad),
-              I(rows), I(cols), Constant(main.inputs.back()), I(lanes)};
-    // A CTA per slice of the load, in warps enough for its tokens.
-    const int64_t slices = LoadSlices(rows);
+    s.args = {In(main.inputs[0]), In(main.inputs[2]), In(main.inputs[1]), Out(part), Out(grad), I(rows), I(cols),
+              Constant(main.inputs[2]), I(lanes)};
+    // A CTA per part of the loss, in warps enough for its tokens.
+    const int64_t parts = BalanceParts(rows), most = per * vec > 16 ? 8 : 16;
     int64_t warps = 1;
-    while (warps < 16 && warps * (32 / lanes) * slices < rows) warps *= 2;
+    while (warps < most && warps * (32 / lanes) * parts < rows) warps *= 2;
     s.block[0] = (unsigned)(32 * warps);
-    s.grid[0]  = (unsigned)slices;
-    s.dyn_smem = (size_t)(load ? warps * cols * 4 : 0);
+    s.grid[0]  = (unsigned)parts;
     steps->push_back(s);
     return true;
   }
@@ -467,21 +453,6 @@ struct LossMatcher {
       zero.block[0] = 256;
       p->steps.push_back(zero);
     }
-    p->steps.push_back(s);
-    return p;
-  }
-
-  std::unique_ptr<CompiledGroup> PlanFold(const OpDesc& op) {
-    const TensorDesc& load = Input(op.inputs[0]);
-    auto p = NewPlan("balance_fold");
-    LaunchStep s;
-    s.kernel = FindKernel("balance_fold");
-    if (!s.kernel) return Fail("kernel balance_fold is missing");
-    s.args     = {In(op.inputs[0]), In(op.inputs[1]), Out(&op), I(load.shape[0]), I(load.shape[1])};
-    const int64_t n = load.numel();
-    s.block[0] = (unsigned)std::max<int64_t>(RoundUp(load.shape[1], 32), std::min<int64_t>(1024, RoundUp(n, 32)));
-    s.cluster  = n > 8192 ? 8 : 0;
-    s.grid[0]  = s.cluster ? s.cluster : 1;
     p->steps.push_back(s);
     return p;
   }

@@ -1,13 +1,18 @@
 // A router's balance loss, its gradient and the per-expert counts.  x is [tokens, experts], w the tokens' weights,
 // c the number of tokens that chose each expert, f = c / sum c; per token q = softmax(x):
 //
-//   loss = E sum_e f_e sum_t w_t q_te        dx_te = w_t E q_te (f_e - sum_e' f_e' q_te')
+//   loss = E sum_t w_t (sum_e f_e q_te)        dx_te = w_t E q_te (f_e - sum_e' f_e' q_te')
 //
-// The gradient needs the counts alone, so it and the column sums of w q share one pass over the logits: the row of a
-// token in the registers of L lanes (L <= 32 lanes, NV vectors of V elements each), the column sums in the same lanes'
-// registers over all tokens of the warp, one partial row per CTA (expert_load), and a small kernel that folds the
-// partial rows and the counts into the loss (balance_fold).  No floating-point atomics: results do not depend on the
-// order of CTAs.  A token of weight 0 is out: it adds nothing and is not read, and its gradient row is 0.
+// The counts come first (they are a constant of the differentiation); loss and gradient then share one pass over the
+// logits, because the sum over the experts that the gradient subtracts is the token's term of the loss: a token's row in
+// the registers of L lanes (NV vectors of V elements each), the terms added up per CTA (balance_part) and then over the
+// CTAs by an ordinary row reduction.  No floating-point atomics: results do not depend on the order of CTAs.  A token of
+// weight 0 is out: it adds nothing and is not read, and its gradient row is 0.
+//
+// Bound by HBM for long batches and, at these row lengths, by instructions nearly as much: three reductions over a token's
+// lanes for eight elements per lane.  Measured with counts, loss and gradient, 65536 x 256 fp32, 8 choices: 28 us (119 MB,
+// 0.65 of the copy bandwidth), of which 8 us are the three small launches around this kernel; 480 us before the row lay
+// in registers as vectors, 34 with 16 elements per lane, 32 with column sums (which the loss does not need) kept too.
 #include <type_traits>
 #include "device_math.cuh"
 #include "kernel_registry.h"
@@ -18,107 +23,158 @@ namespace {
 constexpr int kRouterThreads = 512;
 constexpr int kMaxExperts    = 1024;
 
-// V elements at p, as floats: one vector, or one element.
+// Pairs of floats in one 64-bit register, for the two-wide arithmetic of sm_100.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 pair(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(F2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// What a lane loads at once: a vector of V elements, or one element (V = 1).
 template <typename T, int V>
 struct Raw {
   typedef typename std::conditional<V == 1, T, uint4>::type type;
-};
-template <typename T, int V>
-__device__ __forceinline__ void widen(const typename Raw<T, V>::type& r, float* f) {
-  if constexpr (V == 1) f[0] = Io<T>::load1(&r);
-  else Io<T>::unpack(r, f);
-}
-
-template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kRouterThreads)
-    k_router_loss(const T* __restrict__ x, const float* __restrict__ weight, const int* __restrict__ counts,
-                  float* __restrict__ out_load, T* __restrict__ out_grad, long long rows, long long cols_ll,
-                  double weight_value, long long lanes_ll) {
-  grid_dependency_sync();
-  typedef typename Raw<T, V>::type R;
-  constexpr int K = V * NV;  // elements per lane
-  extern __shared__ float part[];  // [warps][cols]
-  __shared__ float scratch[32];
-  const int cols = (int)cols_ll, L = (int)lanes_ll, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-  const int per_warp = 32 / L, sub = lane & (L - 1), group = lane / L;
-  const int nvec     = cols / V;
-  float f[K], acc[K];
+  __device__ static __forceinline__ void widen(const type& r, float* f) {
+    if constexpr (V == 1) f[0] = Io<T>::load1(&r);
+    else Io<T>::unpack(r, f);
+  }
+  __device__ static __forceinline__ type fill(float v) {
+    if constexpr (V == 1) {
+      T one;
+      Io<T>::store1(&one, v);
+      return one;
+    } else {
+      float f[V];
 #pragma unroll
-  for (int i = 0; i < K; ++i) f[i] = acc[i] = 0.0f;
-  if (out_grad) {
-    // Shares of the choices, less their mean: sum_e q_e = 1, so a constant taken off f changes nothing in
-    // f_e - sum f q but its cancellation.
-    float total = 0.0f;
-    for (int e = threadIdx.x; e < cols; e += blockDim.x) total += (float)counts[e];
-    total = cta_allreduce<SumOp>(total, scratch);
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-      const int v = sub + (i / V) * L;
-      if (v < nvec && total > 0.0f) f[i] = (float)counts[v * V + i % V] / total - 1.0f / (float)cols;
+      for (int i = 0; i < V; ++i) f[i] = v;
+      return Io<T>::pack(f);
     }
   }
+};
+
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThreads)
+    k_router_loss(const T* __restrict__ x, const float* __restrict__ weight, const int* __restrict__ counts,
+                  float* __restrict__ out_part, T* __restrict__ out_grad, long long rows, long long cols_ll,
+                  double weight_value, long long lanes_ll) {
+  grid_dependency_sync();
+  typedef Raw<T, V> Io1;
+  typedef typename Io1::type R;
+  constexpr int K = V * NV;          // elements per lane, a pair at a time (an odd last one is paired with nothing)
+  constexpr int P = (K + 1) / 2;
+  __shared__ float scratch[32];
+  const int cols = (int)cols_ll, L = (int)lanes_ll, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+  const int shift = 31 - __clz(L), per_warp = 32 >> shift, sub = lane & (L - 1), group = lane >> shift;
+  const int nvec  = cols / V;
+  // Shares of the choices, less their mean: sum_e q_e = 1, so a constant taken off f changes nothing in
+  // f_e - sum f q but its cancellation; the loss adds it again.
+  float total = 0.0f, sum = 0.0f;
+  for (int e = threadIdx.x; e < cols; e += blockDim.x) total += (float)counts[e];
+  total             = cta_allreduce<SumOp>(total, scratch);
+  const float scale = total > 0.0f ? 1.0f / total : 0.0f, mean = total > 0.0f ? 1.0f / (float)cols : 0.0f;
+  F2 f[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    float g[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int e = 2 * i + j, v = sub + (e / V) * L;
+      g[j]        = e < K && v < nvec ? fmaf((float)counts[v * V + e % V], scale, -mean) : 0.0f;
+    }
+    f[i] = pair(g[0], g[1]);
+  }
+  // Tokens of this lane's group; the weights are fetched two tokens ahead, the logits one.  A token that is out is not
+  // read: zeros stand for it, and its weight of 0 makes everything it gives 0.
   auto weight_of = [&](long long t) { return t < rows ? (weight ? __ldg(weight + t) : (float)weight_value) : 0.0f; };
   auto load      = [&](long long t, bool on, R (&r)[NV]) {
+    const T* p = x + t * cols + sub * V;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int v = sub + n * L;
-      if (on && v < nvec) {
-        if constexpr (V == 1) r[n] = x[t * cols + v];
-        else r[n] = ld_stream16(x + t * cols + (long long)v * V);
+      if (sub + n * L >= nvec) continue;  // stays minus infinity
+      r[n] = Io1::fill(0.0f);
+      if (on) {
+        if constexpr (V == 1) r[n] = p[n * L];
+        else r[n] = ld_stream16(p + n * L * V);
       }
     }
   };
-  // Tokens of this lane's group; the weights are fetched two tokens ahead, the logits one.
   const long long step = (long long)gridDim.x * W * per_warp;
   long long t = ((long long)blockIdx.x * W + warp) * per_warp + group;
   float w = weight_of(t), w1 = weight_of(t + step);
   R r[NV], r1[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) r[n] = r1[n] = Io1::fill(-INFINITY);
   load(t, w != 0.0f, r);
+  const F2 log2e = pair(1.4426950408889634f, 1.4426950408889634f);
   for (long long base = t - group; base < rows; base += step, t += step) {  // the same trips for all lanes of a warp
     const float w2 = weight_of(t + 2 * step);
     load(t + step, w1 != 0.0f, r1);
-    float q[K], m = -INFINITY, s = 0.0f, inner = 0.0f;
+    float y[2 * P], m = -INFINITY;
+    y[2 * P - 1] = -INFINITY;
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const bool on = w != 0.0f && sub + n * L < nvec;
-      widen<T, V>(r[n], q + n * V);
+    for (int n = 0; n < NV; ++n) Io1::widen(r[n], y + n * V);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (!on) q[n * V + j] = -INFINITY;
-        m = fmaxf(m, q[n * V + j]);
+    for (int i = 0; i < K; ++i) m = fmaxf(m, y[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < L) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    F2 q[P], s2 = pair(0.0f, 0.0f), inner2 = pair(0.0f, 0.0f);
+    const F2 nm = pair(-m, -m);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float a, b;
+      unpair(mul2(add2(pair(y[2 * i], y[2 * i + 1]), nm), log2e), a, b);
+      q[i]   = pair(ex2(a), ex2(b));
+      s2     = add2(s2, q[i]);
+      inner2 = fma2(q[i], f[i], inner2);
+    }
+    float s, inner, lo, hi;
+    unpair(s2, lo, hi);
+    s = lo + hi;
+    unpair(inner2, lo, hi);
+    inner = lo + hi;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < L) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        inner += __shfl_xor_sync(0xffffffffu, inner, o);
       }
+    const float inv = __fdividef(1.0f, s), factor = (float)cols * w * inv;
+    const F2 factor2 = pair(factor, factor), less = pair(-inner * inv, -inner * inv);
+    if (sub == 0) sum = fmaf(w, fmaf(inner, inv, mean), sum);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      unpair(mul2(mul2(factor2, q[i]), add2(f[i], less)), y[2 * i], y[2 * i + 1]);
     }
-    for (int o = L >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base_m = w != 0.0f ? m : 0.0f;
+    if (out_grad && t < rows) {
+      T* p = out_grad + t * cols + sub * V;
 #pragma unroll
-    for (int i = 0; i < K; ++i) {
-      float e;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((q[i] - base_m) * 1.4426950408889634f));
-      q[i] = e;
-      s += e;
-    }
-#pragma unroll
-    for (int i = 0; i < K; ++i) inner = fmaf(q[i], f[i], inner);
-    for (int o = L >> 1; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      inner += __shfl_xor_sync(0xffffffffu, inner, o);
-    }
-    const float inv = 1.0f / s, wq = w != 0.0f ? w * inv : 0.0f;
-    inner *= inv;
-    const float factor = (float)cols * wq;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int v = sub + n * L;
-      float d[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int i = n * V + j;
-        if (w != 0.0f) acc[i] = fmaf(wq, q[i], acc[i]);
-        d[j] = w != 0.0f ? factor * q[i] * (f[i] - inner) : 0.0f;
-      }
-      if (out_grad && t < rows && v < nvec) {
-        if constexpr (V == 1) Io<T>::store1(out_grad + t * cols + v, d[0]);
-        else st_stream16(out_grad + t * cols + (long long)v * V, Io<T>::pack(d));
+      for (int n = 0; n < NV; ++n) {
+        if (sub + n * L >= nvec) continue;
+        if constexpr (V == 1) Io<T>::store1(p + n * L, y[n]);
+        else st_stream16(p + n * L * V, Io<T>::pack(y + n * V));
       }
     }
     w  = w1;
@@ -126,19 +182,9 @@ __global__ void __launch_bounds__(kRouterThreads)
 #pragma unroll
     for (int n = 0; n < NV; ++n) r[n] = r1[n];
   }
-  if (!out_load) return;
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    for (int o = L; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);  // the warp's groups
-    const int v = sub + (i / V) * L;
-    if (group == 0 && v < nvec) part[warp * cols + v * V + i % V] = acc[i];
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < cols; e += blockDim.x) {
-    float v = 0.0f;
-    for (int k = 0; k < W; ++k) v += part[k * cols + e];
-    out_load[(long long)blockIdx.x * cols + e] = v;
-  }
+  if (!out_part) return;
+  sum = cta_allreduce<SumOp>(sum, scratch);
+  if (threadIdx.x == 0) out_part[blockIdx.x] = (float)cols * sum;
 }
 
 // Counts of the choices in shared memory, a thread per token (whole numbers: the order of the additions does not show).
@@ -169,66 +215,10 @@ __global__ void __launch_bounds__(1024) k_expert_zero(int* __restrict__ counts, 
   for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[e] = 0;
 }
 
-// All warps of the cluster, each of them together.
-__device__ __forceinline__ void cluster_barrier() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// loss = E / sum c * sum over slices and experts of c_e load_ke: one flat dot product, over the CTAs of one cluster.
-__global__ void __launch_bounds__(1024)
-    k_balance_fold(const float* __restrict__ load, const int* __restrict__ counts, float* __restrict__ out,
-                   long long slices, long long experts) {
-  grid_dependency_sync();
-  __shared__ float scratch[32];
-  __shared__ float meet[8];
-  int C, rank;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  // A thread keeps to one column, or to four neighbouring ones, and walks down every `down`-th slice.
-  const int E = (int)experts, K = (int)slices, tid = threadIdx.x;
-  const bool four = E % 4 == 0 && (reinterpret_cast<uintptr_t>(load) & 15) == 0;
-  const int across = four ? E / 4 : E, down = blockDim.x / across * C, col = tid % across;
-  const int first = tid / across < blockDim.x / across ? tid / across * C + rank : K;
-  float total = 0.0f, sum = 0.0f;
-  for (int e = tid; e < E; e += blockDim.x) total += (float)counts[e];
-  if (four) {
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int k = first; k < K; k += down) {
-      const float4 u = __ldg(reinterpret_cast<const float4*>(load) + (long long)k * across + col);
-      v[0] += u.x;
-      v[1] += u.y;
-      v[2] += u.z;
-      v[3] += u.w;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum = fmaf((float)counts[4 * col + j], v[j], sum);
-  } else {
-    float v = 0.0f;
-#pragma unroll 8
-    for (int k = first; k < K; k += down) v += __ldg(load + (long long)k * E + col);
-    sum = (float)counts[col] * v;
-  }
-  total = cta_allreduce<SumOp>(total, scratch);
-  sum = cta_allreduce<SumOp>(sum, scratch);
-  if (C > 1) {
-    uint32_t there;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(meet + rank)));
-    cluster_barrier();  // no CTA writes to the first one's shared memory before that one runs
-    if (threadIdx.x == 0) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(sum) : "memory");
-    cluster_barrier();
-    sum = 0.0f;
-    if (rank == 0)
-      for (int k = 0; k < C; ++k) sum += meet[k];
-  }
-  if (rank == 0 && threadIdx.x == 0) out[0] = total > 0.0f ? (float)experts * (sum / total) : 0.0f;
-}
-
 }  // namespace
 
 #define REG_ROUTER(TNAME, T, VN, V, NV) \
-  CINN_B200_REGISTER_KERNEL_PDL("router_loss_" TNAME VN "_n" #NV, 9, kRouterThreads, k_router_loss<T, V, NV>)
+  CINN_B200_REGISTER_KERNEL_PDL("router_loss_" TNAME VN "_n" #NV, 9, V * NV > 16 ? kRouterThreads / 2 : kRouterThreads, k_router_loss<T, V, NV>)
 #define REG_ROUTER_TYPE(TNAME, T, V)   \
   REG_ROUTER(TNAME, T, "_s", 1, 1);    \
   REG_ROUTER(TNAME, T, "_s", 1, 2);    \
@@ -245,6 +235,5 @@ REG_ROUTER_TYPE("f16", __half, 8);
 REG_ROUTER_TYPE("bf16", __nv_bfloat16, 8);
 CINN_B200_REGISTER_KERNEL_PDL("expert_counts", 8, 1024, k_expert_counts);
 CINN_B200_REGISTER_KERNEL_PDL("expert_zero", 2, 1024, k_expert_zero);
-CINN_B200_REGISTER_KERNEL_PDL("balance_fold", 5, 1024, k_balance_fold);
 
 }  // namespace cinn_b200
