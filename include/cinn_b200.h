@@ -138,6 +138,21 @@ int cinn_b200_group_host_chunks(const char* fn_name);
  * a blank-separated "key=value" list with the reference's attribute names (axis, scale, bias,
  * bias_after_scale, dtype, dim, keep_dim, epsilon, data_layout, out_shape, broadcast_axes, shape, value).
  * Output shape and dtype are inferred; the new variable's id is written to id_out.
+ *
+ * Besides the reference's ops, losses over rows of logits and their gradients (row_loss.cu, router_loss.cu).  x = logits
+ * [rows..., columns] fp32 / fp16 / bf16; ids int32 / int64; one fp32 value per row for everything else; results fp32, the
+ * gradients (of the SUM of the losses with respect to the logits) in the logits' type:
+ *     token_logprob       x target                              ; temperature    lp = log softmax(x / temperature)[target]
+ *     token_logprob_grad  x target dlogprob                     ; temperature
+ *     policy_loss[_grad]  x action old ref advantage weight     ; clip_low clip_high kl_coef temperature
+ *         weight (kl_coef (exp(ref - lp) - (ref - lp) - 1) - min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)), r = exp(lp - old)
+ *     distill_loss[_grad] x teacher_logits teacher_index weight ; temperature
+ *         weight sum_k p_k (log p_k - log softmax(x / temperature)[index_k]), p = softmax of the row's kept teacher logits /
+ *         temperature ([rows..., entries <= 1024]; an index outside the columns is an unused entry, one may occur twice)
+ *     expert_counts       index[tokens..., slots] weight        ; num_experts    int32 [num_experts <= 1024]
+ *     balance_loss[_grad] x counts weight        E sum_e counts_e / sum(counts) sum_t weight_t softmax(x_t)_e, E <= 1024 columns
+ * A row of weight 0, or whose token id lies outside the columns, is out: its loss is 0 and its gradient row 0 whatever
+ * else it holds.  The weight (and dlogprob) may be a fill_constant.  Gradients smaller than 2^-126 may come back as 0.
  */
 typedef struct cinn_b200_builder cinn_b200_builder;
 cinn_b200_builder* cinn_b200_builder_create(const char* name);

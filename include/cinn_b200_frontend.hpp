@@ -152,6 +152,41 @@ class NetBuilder {
                      float epsilon = 1e-5f, const std::string& data_layout = "NCHW") {
     return CustomInstr("batch_norm", {x, scale, bias, mean, variance}, "epsilon=" + Num(epsilon) + " data_layout=" + data_layout);
   }
+  // Losses over rows of logits, and the gradients of their sums with respect to the logits (what each computes is
+  // written beside cinn_b200_builder_add_op in cinn_b200.h).  Ops over the same logits run as one kernel.
+  Variable TokenLogprob(const Variable& logits, const Variable& target, float temperature = 1.0f) {
+    return CustomInstr("token_logprob", {logits, target}, "temperature=" + Num(temperature));
+  }
+  Variable TokenLogprobGrad(const Variable& logits, const Variable& target, const Variable& dlogprob, float temperature = 1.0f) {
+    return CustomInstr("token_logprob_grad", {logits, target, dlogprob}, "temperature=" + Num(temperature));
+  }
+#define CINN_B200_POLICY(Name, op)                                                                                         \
+  Variable Name(const Variable& logits, const Variable& action, const Variable& old_logprob, const Variable& ref_logprob,   \
+                const Variable& advantage, const Variable& weight, float clip_low = 0.2f, float clip_high = 0.2f,           \
+                float kl_coef = 0.0f, float temperature = 1.0f) {                                                           \
+    return CustomInstr(op, {logits, action, old_logprob, ref_logprob, advantage, weight},                                   \
+                       "clip_low=" + Num(clip_low) + " clip_high=" + Num(clip_high) + " kl_coef=" + Num(kl_coef) +          \
+                           " temperature=" + Num(temperature));                                                             \
+  }
+  CINN_B200_POLICY(PolicyLoss, "policy_loss") CINN_B200_POLICY(PolicyLossGrad, "policy_loss_grad")
+#undef CINN_B200_POLICY
+  Variable DistillLoss(const Variable& logits, const Variable& teacher_logits, const Variable& teacher_index, const Variable& weight,
+                       float temperature = 1.0f) {
+    return CustomInstr("distill_loss", {logits, teacher_logits, teacher_index, weight}, "temperature=" + Num(temperature));
+  }
+  Variable DistillLossGrad(const Variable& logits, const Variable& teacher_logits, const Variable& teacher_index,
+                           const Variable& weight, float temperature = 1.0f) {
+    return CustomInstr("distill_loss_grad", {logits, teacher_logits, teacher_index, weight}, "temperature=" + Num(temperature));
+  }
+  Variable ExpertCounts(const Variable& index, const Variable& weight, int num_experts) {
+    return CustomInstr("expert_counts", {index, weight}, "num_experts=" + std::to_string(num_experts));
+  }
+  Variable BalanceLoss(const Variable& logits, const Variable& counts, const Variable& weight) {
+    return CustomInstr("balance_loss", {logits, counts, weight});
+  }
+  Variable BalanceLossGrad(const Variable& logits, const Variable& counts, const Variable& weight) {
+    return CustomInstr("balance_loss_grad", {logits, counts, weight});
+  }
   // ProgramPass::Apply (cinn/frontend/program_pass.h:36-105): rewrites the program by the named passes, in order; an
   // empty list applies the default list of cinn/frontend/optimize.cc:44-82.  `fetch` are the variables that must survive.
   void ApplyPasses(const std::vector<Variable>& fetch, const std::vector<std::string>& passes = {}) {

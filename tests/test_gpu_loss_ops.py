@@ -466,6 +466,71 @@ def test_a_constant_weight_equals_a_tensor_of_it():
     assert torch.equal(one["dx"], two["dx"])
 
 
+def test_constant_weights_of_the_other_losses():
+    g, x, a = make(13, 777, "float32")
+    p, t = policy_inputs(g, x, a), distill_inputs(g, x, 9)
+    i = torch.randint(0, 20, (13, 3), generator=g, device="cuda")
+    router = torch.randn(13, 20, generator=g, device="cuda")
+    inputs = {**p, "t": t["t"], "i": t["i"], "g": router, "gi": i}
+    inputs["w"] = torch.full((13,), 0.375, device="cuda")
+
+    def build(weight):
+        def f(b, v):
+            w = v["w"] if weight is None else b.fill_constant([13], weight)
+            args = [v[k] for k in ("x", "a", "old", "ref", "adv")] + [w]
+            c = b.expert_counts(v["gi"], w, 20)
+            return {"pl": b.policy_loss(*args, **POLICY), "pg": b.policy_loss_grad(*args, **POLICY), "c": c,
+                    "dl": b.distill_loss(v["x"], v["t"], v["i"], w), "dg": b.distill_loss_grad(v["x"], v["t"], v["i"], w),
+                    "bl": b.balance_loss(v["g"], c, w), "bg": b.balance_loss_grad(v["g"], c, w)}
+        return f
+    one, two = run_program(build(None), inputs), run_program(build(0.375), inputs)
+    assert all(torch.equal(one[k], two[k]) for k in one)
+    none = run_program(build(0.0), inputs)
+    assert all((none[k] == 0).all() for k in none)
+
+
+def test_a_group_on_host_buffers():
+    rows, cols = 70, 3001
+    g, x, a = make(rows, cols, "float32")
+    w = torch.randn(rows, generator=g, device="cuda")
+    group = cinn_b200.FusedGroup("""group fn_host_logprob
+input x float32 %d,%d
+input a int64 %d
+input w float32 %d
+op token_logprob l = x a
+op token_logprob_grad d = x a w
+output l float32 %d
+output d float32 %d,%d
+""" % (rows, cols, rows, rows, rows, rows, cols))
+    lp, dx = torch.empty(rows, device="cuda"), torch.empty_like(x)
+    group.run([x, a, w, lp, dx])
+    host = [t.cpu().numpy() for t in (x, a, w)] + [torch.zeros(rows).numpy(), torch.zeros(rows, cols).numpy()]
+    group.run_host(host)
+    torch.cuda.synchronize()
+    assert (host[3] == lp.cpu().numpy()).all() and (host[4] == dx.cpu().numpy()).all()
+    group.release()
+
+
+def test_an_exported_program_gives_the_same_bits():
+    g, x, a = make(9, 2500, "float16")
+    inputs = policy_inputs(g, x, a)
+    net = frontend.NetBuilder("exported")
+    v = {k: net.create_input(NAMES[t.dtype], list(t.shape), k) for k, t in inputs.items()}
+    args = [v[k] for k in ("x", "a", "old", "ref", "adv", "w")]
+    out = [net.policy_loss(*args, temperature=0.7, **POLICY), net.policy_loss_grad(*args, temperature=0.7, **POLICY)]
+    comp = frontend.Computation.build_and_compile(common.DefaultNVGPUTarget(), net, fetch=[str(o) for o in out])
+    results = []
+    for c in (comp, frontend.Computation.load(comp.export(), common.DefaultNVGPUTarget())):
+        res = [torch.empty(9, device="cuda"), torch.empty_like(x)]
+        for k, t in inputs.items():
+            c.get_tensor(k).bind(t.data_ptr())
+        for o, t in zip(out, res):
+            c.get_tensor(str(o)).bind(t.data_ptr())
+        c.execute(None)
+        results.append(res)
+    assert all(torch.equal(p, q) for p, q in zip(*results)) and results[0][1].abs().sum() > 0
+
+
 def test_leading_axes_are_rows():
     g, x, a = make(1, 1234, "float16", shape=(3, 5))
     inputs = policy_inputs(g, x, a)

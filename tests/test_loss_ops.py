@@ -1,4 +1,8 @@
 """Loss operators over rows of logits, on the CPU: result types and shapes, refusals, and which ops share a kernel."""
+import os
+import shutil
+import subprocess
+
 import pytest
 
 import cinn_b200
@@ -198,3 +202,38 @@ def test_a_group_whose_operand_has_no_rows_is_refused():
     text = GROUP.format(name="empty", dtype="float32", shape="0,50").replace("4,50", "0,50").replace("int64 4", "int64 0").replace("w float32 4", "w float32 0")
     with pytest.raises(CinnB200Error, match="non-positive extent"):
         cinn_b200.FusedGroup(text)
+
+
+def test_every_per_row_weight_may_be_a_constant():
+    for build in (lambda b, v, w: b.policy_loss(*policy_args(v)[:5], w), lambda b, v, w: b.distill_loss_grad(v["x"], v["t"], v["i"], w),
+                  lambda b, v, w: b.balance_loss_grad(v["g"], v["c"], w), lambda b, v, w: b.expert_counts(v["i"], w, 8)):
+        b, v = net_with()
+        build(b, v, b.fill_constant([6], 0.25))
+        assert len(plan(b)) == 1
+    b, v = net_with()
+    with pytest.raises(CinnB200Error, match="one value per row"):
+        b.policy_loss(*policy_args(v)[:5], b.fill_constant([7], 0.25))
+
+
+@pytest.fixture(scope="module")
+def cpp_program(tmp_path_factory):
+    cinn_b200.lib()
+    gxx = shutil.which("g++")
+    if not gxx:
+        pytest.skip("no g++")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe, libdir = str(tmp_path_factory.mktemp("cpp") / "loss_test"), os.path.join(root, "cinn_b200")
+    subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-I" + os.path.join(root, "include"), os.path.join(root, "tests", "cpp", "loss_test.cc"),
+                    "-o", exe, "-L" + libdir, "-lcinn_b200", "-Wl,-rpath," + libdir], check=True)
+    return exe
+
+
+def test_cpp_front_end_plans_the_losses(cpp_program):
+    out = subprocess.run([cpp_program, "plan"], capture_output=True, text=True)
+    assert out.returncode == 0 and "PLANNED" in out.stdout, out.stdout + out.stderr
+
+
+@pytest.mark.gpu
+def test_cpp_front_end_runs_the_losses(cpp_program):
+    out = subprocess.run([cpp_program, "run"], capture_output=True, text=True)
+    assert out.returncode == 0 and "PASSED" in out.stdout, out.stdout + out.stderr
