@@ -80,8 +80,12 @@ bool InferLossOp(const std::string& op, const std::vector<TensorDesc>& in, std::
   if (in.size() != spec->inputs) return fail("takes " + std::to_string(spec->inputs) + " inputs " + spec->args);
   for (auto& t : in) {
     if (t.shape.empty()) return fail("operands need at least one dimension");
-    for (auto d : t.shape)
+    int64_t n = 1;
+    for (auto d : t.shape) {
       if (d <= 0) return fail("operand '" + t.name + "' has a non-positive extent");
+      if (d > 2147483647 || n > (int64_t{1} << 58) / d) return fail("operand '" + t.name + "' is too large");
+      n *= d;
+    }
   }
   // One value per row of `like` (every axis but the last).
   auto per_row = [&](const TensorDesc& t, const TensorDesc& like, const char* what, DType want) {

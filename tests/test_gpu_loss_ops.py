@@ -247,7 +247,8 @@ def test_policy_loss_and_its_gradient(rows, cols, dtype):
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("rows,cols,k", [(1, 1, 1), (3, 7, 5), (5, 31, 40), (2, 257, 64), (9, 1000, 1), (3, 4097, 33),
-                                         (2, 32768, 1024), (4, 50021, 17), (1, 131072, 64), (301, 2048, 8), (40, 20011, 100)])
+                                         (2, 32768, 1024), (4, 50021, 17), (1, 131072, 64), (301, 2048, 8), (40, 20011, 100), (5, 31, 300), (3, 2000, 1024),
+                                         (700, 129, 128)])
 def test_distill_loss_and_its_gradient(rows, cols, k, dtype):
     tau = 2.0 if rows % 2 else 1.0
     g, x, _ = make(rows, cols, dtype)
@@ -464,6 +465,56 @@ def test_a_constant_weight_equals_a_tensor_of_it():
     one = run_program(lambda b, v: {"dx": b.token_logprob_grad(v["x"], v["a"], v["w"])}, inputs)
     two = run_program(lambda b, v: {"dx": b.token_logprob_grad(v["x"], v["a"], b.fill_constant([11], -0.125))}, inputs)
     assert torch.equal(one["dx"], two["dx"])
+
+
+def test_inputs_that_change_between_runs_without_a_wait():
+    """Runs and copies queued on one stream, none waited for: each run sees the inputs copied in front of it."""
+    rows, cols, experts = 200, 3000, 40
+    sets = []
+    for seed in range(6):
+        g, x, a = make(rows, cols, "bfloat16", seed=seed)
+        p, t = policy_inputs(g, x, a), distill_inputs(g, x, 12)
+        p["w"] = p["w"].roll(seed)
+        router = torch.randn(rows, experts, generator=g, device="cuda")
+        sets.append({**p, "t": t["t"], "i": t["i"], "g": router, "gi": router.topk(3, 1).indices})
+    net = frontend.NetBuilder("changing")
+    v = {k: net.create_input(NAMES[t.dtype], list(t.shape), k) for k, t in sets[0].items()}
+    w = net.scale(v["w"], 0.5)  # computed in the program, by a kernel in front of the losses
+    args = [v[k] for k in ("x", "a", "old", "ref", "adv")] + [w]
+    c = net.expert_counts(v["gi"], w, experts)
+    out = [net.token_logprob(v["x"], v["a"]), net.policy_loss(*args, **POLICY), net.policy_loss_grad(*args, **POLICY),
+           net.distill_loss(v["x"], v["t"], v["i"], w), net.distill_loss_grad(v["x"], v["t"], v["i"], w), c,
+           net.balance_loss(v["g"], c, w), net.balance_loss_grad(v["g"], c, w)]
+    comp = frontend.Computation.build_and_compile(common.DefaultNVGPUTarget(), net, fetch=[str(o) for o in out])
+    kinds = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32}
+    feed = {k: torch.empty_like(t) for k, t in sets[0].items()}
+    res = [torch.empty(o.shape, dtype=kinds[o.type.name], device="cuda") for o in out]
+    for k, t in feed.items():
+        comp.get_tensor(k).bind(t.data_ptr())
+    for o, t in zip(out, res):
+        comp.get_tensor(str(o)).bind(t.data_ptr())
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def run_all(wait):
+        got = []
+        with torch.cuda.stream(stream):
+            for s in sets:
+                for k, t in feed.items():
+                    t.copy_(s[k])
+                if wait:
+                    torch.cuda.synchronize()
+                comp.execute(stream.cuda_stream)
+                if wait:
+                    torch.cuda.synchronize()
+                got.append([t.clone() for t in res])
+        torch.cuda.synchronize()
+        return got
+    want = run_all(True)
+    assert not torch.equal(want[0][5], want[1][5]) and not torch.equal(want[0][1], want[1][1])
+    for _ in range(5):
+        for one, two in zip(run_all(False), want):
+            assert all(torch.equal(p, q) for p, q in zip(one, two))
 
 
 def test_constant_weights_of_the_other_losses():

@@ -198,6 +198,13 @@ def test_a_group_that_mixes_a_loss_with_another_op_is_refused():
         cinn_b200.FusedGroup(text)
 
 
+@pytest.mark.parametrize("rows,cols", [("1", "4294967296"), ("2147483647", "2147483647,2147483647,9")])
+def test_extents_beyond_what_a_buffer_describes_are_refused(rows, cols):
+    text = GROUP.format(name="huge", dtype="float32", shape="4,50").replace("4,50", rows + "," + cols).replace("int64 4", "int64 " + rows).replace("w float32 4", "w float32 " + rows)
+    with pytest.raises(CinnB200Error, match="too large"):
+        cinn_b200.FusedGroup(text)
+
+
 def test_a_group_whose_operand_has_no_rows_is_refused():
     text = GROUP.format(name="empty", dtype="float32", shape="0,50").replace("4,50", "0,50").replace("int64 4", "int64 0").replace("w float32 4", "w float32 0")
     with pytest.raises(CinnB200Error, match="non-positive extent"):
