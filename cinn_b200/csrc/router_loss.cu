@@ -10,9 +10,10 @@
 // weight 0 is out: it adds nothing and is not read, and its gradient row is 0.
 //
 // Bound by HBM for long batches and, at these row lengths, by instructions nearly as much: three reductions over a token's
-// lanes for eight elements per lane.  Measured with counts, loss and gradient, 65536 x 256 fp32, 8 choices: 28 us (119 MB,
-// 0.65 of the copy bandwidth), of which 8 us are the three small launches around this kernel; 480 us before the row lay
-// in registers as vectors, 34 with 16 elements per lane, 32 with column sums (which the loss does not need) kept too.
+// lanes for eight elements per lane.  Measured with counts, loss and gradient, 65536 x 256 fp32, 8 choices: 27 us (119 MB,
+// 0.67 of the copy bandwidth), of which 6 us are the three small launches around this kernel; 480 us before the row lay
+// in registers as vectors, 34 with 16 elements per lane, 32 with column sums (which the loss does not need) kept too, 33 with two tokens
+// per trip (84 registers: one CTA per SM).
 #include <type_traits>
 #include "device_math.cuh"
 #include "kernel_registry.h"
@@ -107,39 +108,49 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
   }
   // Tokens of this lane's group; the weights are fetched two tokens ahead, the logits one.  A token that is out is not
   // read: zeros stand for it, and its weight of 0 makes everything it gives 0.
+  const long long step = (long long)gridDim.x * W * per_warp, jump = step * cols;
+  long long t = ((long long)blockIdx.x * W + warp) * per_warp + group;
+  const T* px = x + t * cols + sub * V;
+  T* pg       = out_grad ? out_grad + t * cols + sub * V : nullptr;
   auto weight_of = [&](long long t) { return t < rows ? (weight ? __ldg(weight + t) : (float)weight_value) : 0.0f; };
-  auto load      = [&](long long t, bool on, R (&r)[NV]) {
-    const T* p = x + t * cols + sub * V;
+  auto load      = [&](const T* p, bool on, R (&r)[NV]) {
+    if (__all_sync(0xffffffffu, on)) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      if (sub + n * L >= nvec) continue;  // stays minus infinity
-      r[n] = Io1::fill(0.0f);
-      if (on) {
-        if constexpr (V == 1) r[n] = p[n * L];
-        else r[n] = ld_stream16(p + n * L * V);
-      }
+      for (int n = 0; n < NV; ++n)
+        if (sub + n * L < nvec) {  // the others stay minus infinity
+          if constexpr (V == 1) r[n] = p[n * L];
+          else r[n] = ld_stream16(p + n * L * V);
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        if (sub + n * L < nvec) {
+          r[n] = Io1::fill(0.0f);
+          if (on) {
+            if constexpr (V == 1) r[n] = p[n * L];
+            else r[n] = ld_stream16(p + n * L * V);
+          }
+        }
     }
   };
-  const long long step = (long long)gridDim.x * W * per_warp;
-  long long t = ((long long)blockIdx.x * W + warp) * per_warp + group;
-  float w = weight_of(t), w1 = weight_of(t + step);
-  R r[NV], r1[NV];
-#pragma unroll
-  for (int n = 0; n < NV; ++n) r[n] = r1[n] = Io1::fill(-INFINITY);
-  load(t, w != 0.0f, r);
-  const F2 log2e = pair(1.4426950408889634f, 1.4426950408889634f);
-  for (long long base = t - group; base < rows; base += step, t += step) {  // the same trips for all lanes of a warp
-    const float w2 = weight_of(t + 2 * step);
-    load(t + step, w1 != 0.0f, r1);
+  const F2 log2e    = pair(1.4426950408889634f, 1.4426950408889634f);
+  const float fcols = (float)cols;
+  // One token: its row is `r`, its weight `w`.
+  auto token = [&](const R (&r)[NV], float w) {
     float y[2 * P], m = -INFINITY;
     y[2 * P - 1] = -INFINITY;
 #pragma unroll
     for (int n = 0; n < NV; ++n) Io1::widen(r[n], y + n * V);
 #pragma unroll
     for (int i = 0; i < K; ++i) m = fmaxf(m, y[i]);
+    if (L == 32) {
+      asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(m));
+    } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      if (o < L) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int o = 8; o > 0; o >>= 1)
+        if (o < L) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (L > 16) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    }
     F2 q[P], s2 = pair(0.0f, 0.0f), inner2 = pair(0.0f, 0.0f);
     const F2 nm = pair(-m, -m);
 #pragma unroll
@@ -150,33 +161,44 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
       s2     = add2(s2, q[i]);
       inner2 = fma2(q[i], f[i], inner2);
     }
-    float s, inner, lo, hi;
-    unpair(s2, lo, hi);
-    s = lo + hi;
-    unpair(inner2, lo, hi);
-    inner = lo + hi;
+    float s0, s1, i0, i1;
+    unpair(s2, s0, s1);
+    unpair(inner2, i0, i1);
+    F2 both = add2(pair(s0, i0), pair(s1, i1));  // the sum of the exponentials and their product with f, side by side
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       if (o < L) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        inner += __shfl_xor_sync(0xffffffffu, inner, o);
+        unpair(both, s0, i0);
+        both = add2(both, pair(__shfl_xor_sync(0xffffffffu, s0, o), __shfl_xor_sync(0xffffffffu, i0, o)));
       }
-    const float inv = __fdividef(1.0f, s), factor = (float)cols * w * inv;
-    const F2 factor2 = pair(factor, factor), less = pair(-inner * inv, -inner * inv);
-    if (sub == 0) sum = fmaf(w, fmaf(inner, inv, mean), sum);
+    unpair(both, s0, i0);
+    const float inv = __fdividef(1.0f, s0), inner = i0 * inv;
+    if (sub == 0) sum = fmaf(w, inner + mean, sum);
+    if (!out_grad) return;
+    const float factor = fcols * w * inv;
+    const F2 factor2 = pair(factor, factor), less = pair(-inner, -inner);
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      unpair(mul2(mul2(factor2, q[i]), add2(f[i], less)), y[2 * i], y[2 * i + 1]);
-    }
-    if (out_grad && t < rows) {
-      T* p = out_grad + t * cols + sub * V;
+    for (int i = 0; i < P; ++i) unpair(mul2(mul2(factor2, q[i]), add2(f[i], less)), y[2 * i], y[2 * i + 1]);
+    if (t < rows) {
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        if (sub + n * L >= nvec) continue;
-        if constexpr (V == 1) Io<T>::store1(p + n * L, y[n]);
-        else st_stream16(p + n * L * V, Io<T>::pack(y + n * V));
-      }
+      for (int n = 0; n < NV; ++n)
+        if (sub + n * L < nvec) {
+          if constexpr (V == 1) Io<T>::store1(pg + n * L, y[n]);
+          else st_stream16(pg + n * L * V, Io<T>::pack(y + n * V));
+        }
     }
+  };
+  float w = weight_of(t), w1 = weight_of(t + step);
+  R r[NV], r1[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) r[n] = r1[n] = Io1::fill(-INFINITY);
+  load(px, w != 0.0f, r);
+  for (long long base = t - group; base < rows; base += step, t += step) {  // the same trips for all lanes of a warp
+    const float w2 = weight_of(t + 2 * step);
+    px += jump;
+    load(px, w1 != 0.0f, r1);
+    token(r, w);
+    pg += jump;
     w  = w1;
     w1 = w2;
 #pragma unroll
