@@ -10,8 +10,8 @@
 // weight 0 is out: it adds nothing and is not read, and its gradient row is 0.
 //
 // Bound by HBM for long batches and, at these row lengths, by instructions nearly as much: three reductions over a token's
-// lanes for eight elements per lane.  Measured with counts, loss and gradient, 65536 x 256 fp32, 8 choices: 27 us (119 MB,
-// 0.67 of the copy bandwidth), of which 6 us are the three small launches around this kernel; 480 us before the row lay
+// lanes for eight elements per lane.  Measured with counts, loss and gradient, 65536 x 256 fp32, 8 choices: 28 us (119 MB,
+// 0.65 of the copy bandwidth), of which 6 us are the three small launches around this kernel; 480 us before the row lay
 // in registers as vectors, 34 with 16 elements per lane, 32 with column sums (which the loss does not need) kept too, 33 with two tokens
 // per trip (84 registers: one CTA per SM).
 #include <type_traits>
@@ -76,7 +76,7 @@ struct Raw {
 };
 
 template <typename T, int V, int NV>
-__global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThreads)
+__global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThreads, V > 1 && (V * NV <= 8 || V * NV == 32) ? 2 : 1)
     k_router_loss(const T* __restrict__ x, const float* __restrict__ weight, const int* __restrict__ counts,
                   float* __restrict__ out_part, T* __restrict__ out_grad, long long rows, long long cols_ll,
                   double weight_value, long long lanes_ll) {
@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
   const int cols = (int)cols_ll, L = (int)lanes_ll, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
   const int shift = 31 - __clz(L), per_warp = 32 >> shift, sub = lane & (L - 1), group = lane >> shift;
   const int nvec  = cols / V;
-  // Shares of the choices, less their mean: sum_e q_e = 1, so a constant taken off f changes nothing in
-  // f_e - sum f q but its cancellation; the loss adds it again.
+  // Shares of the choices.  In f_e - sum f q a constant may be taken off f, because sum q = 1: less their mean, shares
+  // that are nearly alike do not cancel.  The loss is summed without that, and by lanes: its terms are all positive.
   float total = 0.0f, sum = 0.0f;
   for (int e = threadIdx.x; e < cols; e += blockDim.x) total += (float)counts[e];
   total             = cta_allreduce<SumOp>(total, scratch);
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int e = 2 * i + j, v = sub + (e / V) * L;
-      g[j]        = e < K && v < nvec ? fmaf((float)counts[v * V + e % V], scale, -mean) : 0.0f;
+      g[j]        = e < K && v < nvec ? (float)counts[v * V + e % V] * scale : 0.0f;
     }
     f[i] = pair(g[0], g[1]);
   }
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
   };
   const F2 log2e    = pair(1.4426950408889634f, 1.4426950408889634f);
   const float fcols = (float)cols;
+  const F2 less_mean = pair(-mean, -mean);
   // One token: its row is `r`, its weight `w`.
   auto token = [&](const R (&r)[NV], float w) {
     float y[2 * P], m = -INFINITY;
@@ -151,18 +152,29 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
         if (o < L) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (L > 16) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
     }
-    F2 q[P], s2 = pair(0.0f, 0.0f), inner2 = pair(0.0f, 0.0f);
+    F2 q[P], s2 = pair(0.0f, 0.0f), dot2 = pair(0.0f, 0.0f), inner2 = pair(0.0f, 0.0f);
     const F2 nm = pair(-m, -m);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       float a, b;
       unpair(mul2(add2(pair(y[2 * i], y[2 * i + 1]), nm), log2e), a, b);
-      q[i]   = pair(ex2(a), ex2(b));
-      s2     = add2(s2, q[i]);
-      inner2 = fma2(q[i], f[i], inner2);
+      q[i] = pair(ex2(a), ex2(b));
+      s2   = add2(s2, q[i]);
+      dot2 = fma2(q[i], f[i], dot2);
     }
-    float s0, s1, i0, i1;
+    float s0, s1, i0, i1, d0, d1;
     unpair(s2, s0, s1);
+    unpair(dot2, d0, d1);
+    if (!out_grad) {
+      s0 += s1;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        if (o < L) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+      sum = fmaf(w, (d0 + d1) * __fdividef(1.0f, s0), sum);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) inner2 = fma2(q[i], add2(f[i], less_mean), inner2);
     unpair(inner2, i0, i1);
     F2 both = add2(pair(s0, i0), pair(s1, i1));  // the sum of the exponentials and their product with f, side by side
 #pragma unroll
@@ -172,13 +184,13 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
         both = add2(both, pair(__shfl_xor_sync(0xffffffffu, s0, o), __shfl_xor_sync(0xffffffffu, i0, o)));
       }
     unpair(both, s0, i0);
-    const float inv = __fdividef(1.0f, s0), inner = i0 * inv;
-    if (sub == 0) sum = fmaf(w, inner + mean, sum);
-    if (!out_grad) return;
+    const float inv = __fdividef(1.0f, s0), less_inner = -i0 * inv;
+    sum = fmaf(w, (d0 + d1) * inv, sum);
     const float factor = fcols * w * inv;
-    const F2 factor2 = pair(factor, factor), less = pair(-inner, -inner);
+    const F2 factor2 = pair(factor, factor), less = pair(less_inner, less_inner);
 #pragma unroll
-    for (int i = 0; i < P; ++i) unpair(mul2(mul2(factor2, q[i]), add2(f[i], less)), y[2 * i], y[2 * i + 1]);
+    for (int i = 0; i < P; ++i)
+      unpair(mul2(mul2(factor2, q[i]), add2(add2(f[i], less_mean), less)), y[2 * i], y[2 * i + 1]);
     if (t < rows) {
 #pragma unroll
       for (int n = 0; n < NV; ++n)

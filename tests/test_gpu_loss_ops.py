@@ -267,7 +267,7 @@ def test_distill_loss_and_its_gradient(rows, cols, k, dtype):
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("rows,experts,k", [(1, 1, 1), (1, 2, 1), (7, 3, 3), (64, 16, 2), (65, 61, 4), (1000, 128, 8),
-                                            (4099, 256, 8), (333, 1024, 2), (20000, 60, 6), (513, 511, 1)])
+                                            (4099, 256, 8), (333, 1024, 2), (20000, 60, 6), (513, 511, 1), (2, 6, 5), (1, 627, 1), (2, 57, 5), (8, 4, 1)])
 def test_balance_loss_its_gradient_and_the_counts(rows, experts, k, dtype):
     g, x, _ = make(rows, experts, dtype)
     i = torch.randint(0, experts, (rows, k), generator=g, device="cuda", dtype=torch.int32 if rows % 2 else torch.int64)
