@@ -211,6 +211,17 @@ __device__ __forceinline__ void bulk_load_hint(void* smem_dst, const void* gmem_
                "l"(gmem_src), "r"(bytes), "r"(smem_addr(bar)), "l"(policy)
                : "memory");
 }
+// Asks for [from, to) in L2.  A hint: nothing is read, so it need not wait for the kernel before this one, which may still
+// be writing there.
+__device__ __forceinline__ void hint_l2(const void* from, const void* to) {
+  const uintptr_t a = (reinterpret_cast<uintptr_t>(from) + 15) & ~(uintptr_t)15, b = reinterpret_cast<uintptr_t>(to) & ~(uintptr_t)15;
+  if (b > a) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"((uint32_t)(b - a)) : "memory");
+}
+__device__ __forceinline__ unsigned sm_count() {
+  unsigned n;
+  asm("mov.u32 %0, %%nsmid;" : "=r"(n));
+  return n;
+}
 // All warps of the cluster, each of them together.
 __device__ __forceinline__ void cluster_barrier() {
   __syncwarp();
@@ -315,6 +326,30 @@ __device__ __forceinline__ void keep_entries(const Call<T>& o, long long row, co
     k.t[n]            = good ? t : -INFINITY;
     k.x[n]            = good ? Io<T>::load1(o.x + row * o.cols + i) : 0.0f;
   }
+}
+// The same with one entry per thread, fetched early: its column and logit when the row begins, the student's logit there
+// (which needs the column) while the row is being read, stored once the row has been.
+struct EarlyEntry {
+  long long id;
+  float t, x;
+};
+template <typename T>
+__device__ __forceinline__ EarlyEntry fetch_entry(const Call<T>& o, long long row, int thread) {
+  if (thread >= o.entries) return {-2, 0.0f, 0.0f};
+  const long long at = row * o.entries + thread;
+  return {load_index(o.ids, at, o.wide), load_float(o.a0, at, o.teacher), 0.0f};
+}
+template <typename T>
+__device__ __forceinline__ void fetch_student(const Call<T>& o, const T* xr, int thread, EarlyEntry& e) {
+  const bool good = e.id >= 0 && e.id < o.cols;
+  if (good) e.x = Io<T>::load1(xr + e.id);
+  else if (thread < o.entries) e.id = -1, e.t = -INFINITY;
+}
+__device__ __forceinline__ void keep_entry(const Kept& k, int thread, const EarlyEntry& e) {
+  if (thread >= k.padded) return;
+  k.id[thread] = (int)e.id;
+  k.t[thread]  = e.t;
+  k.x[thread]  = e.x;
 }
 template <typename T>
 __device__ __forceinline__ void prefetch_entries(const Call<T>& o, long long row, int thread, int threads) {
@@ -458,7 +493,6 @@ __device__ __forceinline__ void barrier_of(int group, int threads) {
 
 template <typename T, int KIND, bool GRAD>
 __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PARAMS, long long slots_ll) {
-  grid_dependency_sync();
   constexpr int V = 16 / sizeof(T);
   extern __shared__ __align__(128) unsigned char smem[];
   const Call<T> o = ROW_LOSS_CALL;
@@ -474,8 +508,24 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
   uint64_t* met   = empty + N;                           // completes when the pairs of all G warps are here
   float2* meet    = reinterpret_cast<float2*>(met + 1);  // [G]
   const T* xr     = x + row * cols;
-  const Head h    = head_of<T, KIND, GRAD>(o, row);
   const Row r     = row_at(x, row, o.cols, rank, C);
+  const int chunk = T32 * kUnroll;  // vectors of a slot
+  const bool producer = warp == W;
+  // While the kernel before this one ends: barriers, and the first wave's rows into L2 (1000 x 50021 fp16 with the gradient
+  // 41 -> 39 us back to back).
+  if (producer && lane == 0) {
+    for (int s = 0; s < N; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], W);
+    }
+    mbar_init(met, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (C > 1) mbar_arrive_expect_tx(met, (uint32_t)G * 8u);
+    const char* p = r.body + (size_t)r.start * 16;
+    if (blockIdx.x < 3 * sm_count()) hint_l2(p, p + (size_t)min(r.count, N * chunk) * 16);
+  }
+  grid_dependency_sync();
+  const Head h    = head_of<T, KIND, GRAD>(o, row);
   const int edge  = edge_of(r, o.cols, g == 0, lane);
   T* gr           = GRAD ? out_grad + row * cols : nullptr;
   char* body      = GRAD ? reinterpret_cast<char*>(gr + r.head) + (size_t)r.start * 16 : nullptr;
@@ -491,11 +541,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
     return;
   }
 
-  const int chunk  = T32 * kUnroll;                          // vectors of a slot
   const int chunks = (r.count + chunk - 1) / chunk;
   const int held   = GRAD ? min(chunks, N) : 0;              // pass 2 finds the last ones still in the ring
   const int total  = GRAD ? 2 * chunks - held : chunks;      // and has the others fetched again, last one first
-  const bool producer = warp == W;
   auto copy = [&](int i, int s) {
     const int at         = (i < chunks ? i : total - 1 - i) * chunk;
     const uint32_t bytes = (uint32_t)min(r.count - at, chunk) * 16u;
@@ -503,16 +551,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
     bulk_load_hint(smem + (size_t)s * slot_bytes, r.body + (size_t)(r.start + at) * 16, bytes, &full[s],
                    i < total - chunks ? l2_keep() : l2_pass());
   };
-  if (producer && lane == 0) {
-    for (int s = 0; s < N; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], W);
-    }
-    mbar_init(met, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (C > 1) mbar_arrive_expect_tx(met, (uint32_t)G * 8u);
+  if (producer && lane == 0)
     for (int i = 0; i < min(N, total); ++i) copy(i, i);
-  }
   __syncwarp();
   __syncthreads();
   if (C > 1) cluster_barrier();  // no CTA writes to another's shared memory before that one runs
@@ -541,7 +581,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
   if (edge >= 0) xe = Io<T>::load1(xr + edge);
   if (KIND != kDistill) xa = Io<T>::load1(xr + h.a);
   const PolicyOperands po = policy_operands<T, KIND>(o, row);
-  if (KIND == kDistill) prefetch_entries(o, row, tid, T32);  // they are wanted after pass 1
+  EarlyEntry entry = {-2, 0.0f, 0.0f};
+  if (KIND == kDistill) {
+    if (o.entries <= T32) {
+      entry = fetch_entry(o, row, tid);
+      fetch_student(o, xr, tid, entry);
+    } else {
+      prefetch_entries(o, row, tid, T32);  // they are fetched after pass 1
+    }
+  }
 
   // Pass 1.
   Walk k   = start_walk(xe, o.c);
@@ -580,7 +628,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
     next_slot();
   }
   Sum t = end_walk(k, o.c);
-  if (KIND == kDistill) keep_entries(o, row, kept, tid, T32);  // for every warp of this CTA
+  if (KIND == kDistill) {  // for every warp of this CTA
+    if (o.entries <= T32) keep_entry(kept, tid, entry);
+    else keep_entries(o, row, kept, tid, T32);
+  }
   if (G > 1) {
     if (C == 1) {
       if (lane == 0) meet[warp] = make_float2(t.m, t.s);
@@ -658,6 +709,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
 // of them loaded at once.  A row's warps meet at a barrier of their own.
 template <typename T, int KIND, bool GRAD, int NV>
 __global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOSS_PARAMS, long long shift_ll) {
+  if (threadIdx.x == 0 && blockIdx.x < 4 * sm_count()) {  // the first wave's rows into L2 while the kernel before this one ends
+    const long long first = (long long)blockIdx.x * (8 >> (int)shift_ll);
+    hint_l2(x + first * cols, x + min(rows, first + (8 >> (int)shift_ll)) * cols);
+  }
   grid_dependency_sync();
   constexpr int V = 16 / sizeof(T);
   extern __shared__ __align__(128) unsigned char smem[];
@@ -684,6 +739,8 @@ __global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOS
     }
     return;
   }
+  EarlyEntry entry = {-2, 0.0f, 0.0f};
+  if (KIND == kDistill && o.entries <= T32) entry = fetch_entry(o, row, tid);
   uint4 u[NV];
   const uint4* src = reinterpret_cast<const uint4*>(r.body) + tid;
 #pragma unroll
@@ -692,7 +749,10 @@ __global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOS
   if (edge >= 0) xe = Io<T>::load1(xr + edge);
   if (KIND != kDistill) xa = Io<T>::load1(xr + h.a);
   const PolicyOperands po = policy_operands<T, KIND>(o, row);
-  if (KIND == kDistill) keep_entries(o, row, kept, tid, T32);
+  if (KIND == kDistill) {
+    if (o.entries <= T32) fetch_student(o, xr, tid, entry);
+    else keep_entries(o, row, kept, tid, T32);
+  }
   Walk k = start_walk(xe, o.c);
   if constexpr (NV == 8) {
     walk<T, 4>(reinterpret_cast<const uint4(&)[4]>(u[0]), o.c, o.margin, k);
@@ -701,6 +761,7 @@ __global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOS
     walk<T, NV>(u, o.c, o.margin, k);
   }
   Sum t = end_walk(k, o.c);
+  if (KIND == kDistill && o.entries <= T32) keep_entry(kept, tid, entry);
   if (W > 1) {
     if (lane == 0) meet[group * W + warp] = make_float2(t.m, t.s);
     barrier_of(group, T32);
