@@ -9,8 +9,9 @@
 //   distill_loss    p = softmax over the row's teacher entries / temperature
 //                   loss = w sum_k p_k (log p_k - log q_{i_k}),   dx_j = w / temperature * (q_j - sum_{i_k = j} p_k)
 //
-// A row whose weight is 0, whose token id lies outside [0, cols), or whose teacher entries are all outside is out: its
-// loss is 0 and its gradient row 0 whatever its operands hold, and it is not read.  token_logprob needs no weight.
+// A row whose weight is 0, whose token id lies outside [0, cols), or whose teacher entries are all outside or -infinity is
+// out: its loss is 0 and its gradient row 0 whatever its operands hold (in the first two cases it is not read).
+// token_logprob needs no weight.
 //
 // What bounds it: HBM.  A logit is read once and its gradient written once, 2 to 8 bytes for about ten instructions,
 // one or two of them exponentials (at 16 bits those alone take three quarters of the special-function units' rate).
@@ -387,16 +388,21 @@ __device__ __forceinline__ Terms row_terms(const Call<T>& o, long long row, cons
     k.coef = -k.slope * o.inv_t;
     return k;
   }
-  for (int n = lane; n < o.entries; n += 32) k.tmax = fmaxf(k.tmax, kept.t[n]);
+  bool nan = false;  // the maxima pass over it
+  for (int n = lane; n < o.entries; n += 32) {
+    const float v = kept.t[n];
+    k.tmax        = fmaxf(k.tmax, v);
+    nan |= v != v;
+  }
   k.tmax = warp_max(k.tmax);
-  k.live = k.tmax > -INFINITY;  // otherwise the teacher keeps nothing, and the row is out
+  k.live = __any_sync(0xffffffffu, nan) || k.tmax > -INFINITY;  // otherwise the teacher keeps nothing, and the row is out
   for (int n = lane; n < o.entries && k.live; n += 32) k.tsum += ex2((kept.t[n] - k.tmax) * o.c);
   k.tsum = warp_allreduce<SumOp>(k.tsum);
   if (o.out_loss && sums) {
     const float lt = log2f(k.tsum);
     for (int n = lane; n < o.entries && k.live; n += 32) {
       const float lp2 = (kept.t[n] - k.tmax) * o.c - lt, p = ex2(lp2);
-      if (p > 0.0f) loss += p * (lp2 * 0.6931471805599453f - logq(kept.x[n]));
+      if (p != 0.0f) loss += p * (lp2 * 0.6931471805599453f - logq(kept.x[n]));
     }
     loss = warp_allreduce<SumOp>(loss);
     if (lane == 0) o.out_loss[row] = k.live ? h.w * loss : 0.0f;

@@ -421,7 +421,8 @@ class NetBuilder:
         """Divergence of the student's softmax from a teacher known by its top logits: [rows..., entries] logits and
         the columns they belong to (outside [0, columns): an unused entry; a column may occur more than once).  With
         p = softmax over the row's used entries of teacher_logits / temperature and q = softmax(logits / temperature),
-        weight * sum_k p_k (log p_k - log q[index_k]) per row, float32.  At most 1024 entries."""
+        weight * sum_k p_k (log p_k - log q[index_k]) per row, float32; 0 where no used entry is above -infinity.  At
+        most 1024 entries."""
         return self._op("distill_loss", [logits, teacher_logits, teacher_index, weight], temperature=float(temperature))
 
     def distill_loss_grad(self, logits, teacher_logits, teacher_index, weight, temperature=1.0):

@@ -417,6 +417,27 @@ def test_teacher_entries_outside_repeated_or_masked():
     check_grad(got["dx"], want["dlogits"], 0.5 * (want["q"] + want["mass"]), d[:, None], "dlogits")
 
 
+@pytest.mark.parametrize("cols,k", [(40, 1), (40, 5), (3000, 33), (3000, 200), (40000, 1), (40000, 5), (40000, 300)])
+@pytest.mark.parametrize("bad", [float("nan"), INF])
+def test_a_teacher_of_nan_or_infinity_gives_nan_in_its_row_alone(cols, k, bad):
+    g, x, _ = make(5, cols, "float32")
+    inputs = distill_inputs(g, x, k)
+    inputs["w"][:] = 1.0
+    i, t = inputs["i"], inputs["t"]
+    i[:] = torch.randperm(cols, generator=g, device="cuda")[:k] if k <= cols else i
+    t[1, k - 1] = bad             # among other entries
+    t[2], i[2] = -INF, -1         # alone: the others are unused
+    t[2, 0], i[2, 0] = bad, 3
+    t[3, k // 2], i[3, k // 2] = bad, cols  # outside: not used
+    got = run_program(lambda b, v: {"loss": b.distill_loss(v["x"], v["t"], v["i"], v["w"]),
+                                    "dx": b.distill_loss_grad(v["x"], v["t"], v["i"], v["w"])}, inputs)
+    used = torch.zeros(5, cols, dtype=torch.bool, device="cuda")
+    used[1, i[1].long()] = True
+    used[2, 3] = True
+    assert torch.isnan(got["loss"]).tolist() == [False, True, True, False, False]
+    assert torch.equal(torch.isnan(got["dx"]), used)
+
+
 def test_policy_without_kl_reads_no_reference():
     g, x, a = make(5, 3001, "float32")
     inputs = policy_inputs(g, x, a)
