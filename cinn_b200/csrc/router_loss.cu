@@ -221,28 +221,83 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
   if (threadIdx.x == 0) out_part[blockIdx.x] = (float)cols * sum;
 }
 
-// Counts of the choices in shared memory, a thread per token (whole numbers: the order of the additions does not show).
-// One CTA writes the result; several add to one that k_expert_zero has cleared.
+// All warps of the cluster, each of them together.
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Adds this thread's choices to the CTA's bins, eight read before the first is counted (compared as they come, each load
+// waited for the one before: 16384 x 4 choices on 8 CTAs 5.5 us, now 4.2).  Neighbouring threads take neighbouring choices.
+// There are fewer than 2^31 choices and at most 2^17 threads: 32 bits hold every position.  Bins per lane, without bank
+// conflicts, are no faster (5.1 us).
+template <class Index>
+__device__ __forceinline__ void count_choices(int* bins, const Index* __restrict__ index, const float* __restrict__ weight,
+                                              float weight_value, unsigned n, unsigned slots, unsigned experts) {
+  constexpr int kAhead = 8;
+  const unsigned step = gridDim.x * blockDim.x, step_t = step / slots, step_s = step - step_t * slots;
+  unsigned i = blockIdx.x * blockDim.x + threadIdx.x, t = i / slots, s = i - t * slots;
+  while (i < n) {
+    Index chosen[kAhead];
+    float w[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      chosen[u] = -1;
+      w[u]      = weight_value;
+      if (i < n) {
+        chosen[u] = __ldg(index + i);
+        if (weight) w[u] = __ldg(weight + t);
+      }
+      i += step;
+      t += step_t;
+      s += step_s;
+      if (s >= slots) {
+        s -= slots;
+        ++t;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (w[u] != 0.0f && chosen[u] >= 0 && chosen[u] < (Index)experts) atomicAdd(&bins[(int)chosen[u]], 1);
+  }
+}
+
+// Counts of the choices in shared memory (whole numbers: the order of the additions does not show).  The CTAs of one
+// cluster add up each other's bins and write the result; the CTAs of a larger grid add theirs to one that k_expert_zero
+// has cleared.
 __global__ void __launch_bounds__(1024)
     k_expert_counts(const void* __restrict__ index, const float* __restrict__ weight, int* __restrict__ counts,
-                    long long rows, long long slots, long long experts, long long wide, double weight_value) {
+                    long long choices, long long slots, long long experts, long long wide, double weight_value) {
   grid_dependency_sync();
   __shared__ int bins[kMaxExperts];
+  int C, rank;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   for (int e = threadIdx.x; e < experts; e += blockDim.x) bins[e] = 0;
   __syncthreads();
-  for (long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x; t < rows; t += (long long)gridDim.x * blockDim.x) {
-    if ((weight ? __ldg(weight + t) : (float)weight_value) == 0.0f) continue;
-#pragma unroll 4
-    for (long long i = t * slots; i < (t + 1) * slots; ++i) {
-      const long long e = wide ? __ldg(reinterpret_cast<const long long*>(index) + i) : (long long)__ldg(reinterpret_cast<const int*>(index) + i);
-      if (e >= 0 && e < experts) atomicAdd(&bins[e], 1);
-    }
-  }
+  if (wide) count_choices(bins, static_cast<const long long*>(index), weight, (float)weight_value, choices, slots, experts);
+  else count_choices(bins, static_cast<const int*>(index), weight, (float)weight_value, choices, slots, experts);
   __syncthreads();
-  for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-    if (gridDim.x == 1) counts[e] = bins[e];
-    else if (bins[e]) atomicAdd(counts + e, bins[e]);
+  if (gridDim.x > C) {
+    for (int e = threadIdx.x; e < experts; e += blockDim.x)
+      if (bins[e]) atomicAdd(counts + e, bins[e]);
+    return;
   }
+  if (C > 1) cluster_barrier();  // every CTA's bins are complete
+  for (int e = rank * blockDim.x + threadIdx.x; e < experts; e += C * blockDim.x) {
+    const unsigned mine = (unsigned)__cvta_generic_to_shared(bins + e);
+    int sum             = 0;
+    for (int c = 0; c < C; ++c) {
+      unsigned there;
+      int v;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(mine), "r"(c));
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
+      sum += v;
+    }
+    counts[e] = sum;
+  }
+  if (C > 1) cluster_barrier();  // no CTA leaves while another reads its bins
 }
 __global__ void __launch_bounds__(1024) k_expert_zero(int* __restrict__ counts, long long experts) {
   grid_dependency_sync();

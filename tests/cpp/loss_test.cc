@@ -39,7 +39,7 @@ int main(int argc, char** argv) {
       printf("group: %s\n", p.c_str());
       rows += p.find("row_loss") == 0;
     }
-    if (rows != 3 || comp->GroupPatterns().size() != 6) {
+    if (rows != 3 || comp->GroupPatterns().size() != 5) {
       printf("FAILED: the loss ops were not merged as expected\n");
       return 1;
     }

@@ -61,11 +61,12 @@ def test_ops_over_one_tensor_of_logits_share_a_kernel():
     b.distill_loss_grad(v["x"], v["t"], v["i"], v["w"])
     b.distill_loss(v["x"], v["t"], v["i"], v["w"])
     assert plan(b) == ["row_loss"]
-    b, v = net_with()
-    c = b.expert_counts(v["i"], v["w"], 8)
-    b.balance_loss(v["g"], c, v["w"])
-    b.balance_loss_grad(v["g"], c, v["w"])
-    assert sorted(plan(b)) == ["expert_counts", "router_loss", "row_reduce"]
+    for rows, groups in ((65,), ["expert_counts", "router_loss", "row_reduce"]), ((64,), ["expert_counts", "router_loss"]):
+        b, v = net_with(rows)
+        c = b.expert_counts(v["i"], v["w"], 8)
+        b.balance_loss(v["g"], c, v["w"])
+        b.balance_loss_grad(v["g"], c, v["w"])
+        assert sorted(plan(b)) == groups
 
 
 def test_ops_that_differ_stay_apart():
