@@ -14,10 +14,11 @@
 
 namespace cinn_b200 {
 
-// First statement of the kernels that may be launched with programmatic stream serialisation: wait until the
-// kernel launched before this one on the stream has completed and its writes are visible (a no-op for an ordinary
-// launch), then allow the NEXT kernel of the stream to be scheduled early in turn.  The dependents are released only
-// after this wait, so at most one kernel ever sits waiting behind a running one.
+// Stands before the first read or write of global memory in the kernels that may be launched with programmatic stream
+// serialisation (what may come earlier: KernelEntry::pdl, kernel_registry.h): wait until the kernel launched before this
+// one on the stream has completed and its writes are visible (a no-op for an ordinary launch), then allow the NEXT kernel
+// of the stream to be scheduled early in turn.  The dependents are released only after this wait, so at most one kernel
+// ever sits waiting behind a running one.
 __device__ __forceinline__ void grid_dependency_sync() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -17,8 +17,10 @@ struct KernelEntry {
   const void* fn;     // host stub address, what cinn_call_cuda_kernel receives as kernel_fn
   int num_params;     // number of kernel parameters (pointers first, then scalars)
   int max_threads;    // __launch_bounds__ of the kernel
-  bool pdl;           // the kernel calls grid_dependency_sync() before it touches global memory, so it may be
-                      // launched with programmatic stream serialisation (see LaunchEntry in runtime.cc)
+  bool pdl;           // the kernel reads and writes global memory only after grid_dependency_sync(), so it may be
+                      // launched with programmatic stream serialisation (see LaunchEntry in runtime.cc).  What may
+                      // stand before it: work on its own shared memory (mbarriers, the barrier by which a cluster's
+                      // CTAs learn that all of them run) and hints that bring operands into L2.
 };
 
 // Adds an entry at static-initialisation time; returns its index.
@@ -55,7 +57,7 @@ int NumStaticChains();
   static ::cinn_b200::KernelRegistrar CINN_B200_CAT(cinn_b200_kernel_registrar_, __COUNTER__)(        \
       name, reinterpret_cast<const void*>(&__VA_ARGS__), num_params, max_threads)
 
-// The same for a kernel whose first statement is grid_dependency_sync().
+// The same for a kernel that keeps to the rule beside KernelEntry::pdl.
 #define CINN_B200_REGISTER_KERNEL_PDL(name, num_params, max_threads, ...)                              \
   static ::cinn_b200::KernelRegistrar CINN_B200_CAT(cinn_b200_kernel_registrar_, __COUNTER__)(        \
       name, reinterpret_cast<const void*>(&__VA_ARGS__), num_params, max_threads, true)

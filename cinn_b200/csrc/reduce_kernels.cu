@@ -123,10 +123,14 @@ template <class Op>
 __global__ void __launch_bounds__(512) k_row_reduce_cluster(const float* __restrict__ x, float* __restrict__ y,
                                                             long long rows, long long r, long long seg,
                                                             long long vec_ok) {
-  grid_dependency_sync();
   __shared__ float scratch[32];
   __shared__ float partials[16];
-  cg::cluster_group cluster  = cg::this_cluster();
+  cg::cluster_group cluster = cg::this_cluster();
+  // A CTA's shared memory may be written by another only once that CTA is known to run: the CTAs of a cluster are
+  // scheduled together but need not start together.  (No global memory is touched, so this comes in front of the wait
+  // for the kernel before.)
+  cluster.sync();
+  grid_dependency_sync();
   const unsigned rank        = cluster.block_rank();
   const unsigned csize       = cluster.num_blocks();
   const long long n_clusters = gridDim.x / csize;

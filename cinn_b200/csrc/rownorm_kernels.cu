@@ -227,11 +227,13 @@ __global__ void __launch_bounds__(512)
     k_rownorm_cluster(const T* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta,
                       T* __restrict__ y, long long rows, long long cols, long long seg, long long mode,
                       double eps_d) {
-  grid_dependency_sync();
   extern __shared__ __align__(16) float row_smem[];
   __shared__ float scratch[32];
   __shared__ float part1[16], part2[16];
-  cg::cluster_group cluster  = cg::this_cluster();
+  cg::cluster_group cluster = cg::this_cluster();
+  // No CTA writes to a peer's part1 / part2 before that peer is known to run (as in k_row_reduce_cluster).
+  cluster.sync();
+  grid_dependency_sync();
   const unsigned rank        = cluster.block_rank();
   const unsigned csize       = cluster.num_blocks();
   const long long n_clusters = gridDim.x / csize;

@@ -222,7 +222,8 @@ static int LaunchEntry(const KernelEntry* entry, void* v_args, int num_args, int
     // Programmatic dependent launch: the kernel may be scheduled while the previous kernel of the stream is still
     // draining; it blocks in grid_dependency_sync() (griddepcontrol.wait) until that kernel has completed and its
     // writes are visible, so the stream's ordering is kept and only the launch latency is hidden.  Short launches
-    // (a shard of a group on one of eight GPUs runs 5-15 us) gain 1-2 us each.
+    // (a shard of a group on one of eight GPUs runs 5-15 us) gain 1-2 us each; cluster launches too (B200, back to back:
+    // row sums of 40 x 70000 fp32 13.4 -> 10.7 us, softmax of 6 x 100000 13.3 -> 11.3).
     cudaLaunchAttribute& a                       = attr[cfg.numAttrs++];
     a.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
     a.val.programmaticStreamSerializationAllowed = 1;
