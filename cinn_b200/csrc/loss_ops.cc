@@ -342,7 +342,7 @@ struct LossMatcher {
     for (int64_t v : {rows, cols, entries, wide, teacher}) s.args.push_back(I(v));
     s.args.push_back(weight < 0 ? F(0.0) : Constant(main.inputs[weight]));
     const double t = Attr(main, "temperature"), c = 1.4426950408889634 / t;  // exp(z / t) = 2^(c z)
-    for (double v : {1.0 / t, c, 24.0 / c}) s.args.push_back(F(v));
+    for (double v : {1.0 / t, c}) s.args.push_back(F(v));
     s.args.push_back(F(kind == 1 ? 1.0 - Attr(main, "clip_low") : 0.0));
     s.args.push_back(F(kind == 1 ? 1.0 + Attr(main, "clip_high") : 0.0));
     s.args.push_back(F(kind == 1 ? Attr(main, "kl_coef") : 0.0));

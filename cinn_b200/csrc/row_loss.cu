@@ -17,12 +17,12 @@
 // one or two of them exponentials (at 16 bits those alone take three quarters of the special-function units' rate).
 // Layout: a row belongs to one CTA, or to a cluster of C CTAs when there are few rows.  A CTA has W warps that compute
 // and one whose first lane brings the row's 16-byte vectors through a ring of N shared-memory slots (four vectors per
-// computing thread each) with bulk asynchronous copies.  Pass 1 keeps a running reference and sum per lane; the warps'
-// (reference, sum) pairs meet once, in shared memory or in distributed shared memory across the cluster.  Pass 2 turns
-// the row into its gradient: first the last chunks, which are still in the ring, then the others, which come through
-// the ring again from L2, the last one first.  Copies that will be wanted again ask L2 to keep them (evict_last), the
-// others let go (evict_first).  CTAs are not persistent: the hardware deals rows to SMs as they come free, which rows
-// that are out make uneven, and co-resident CTAs cover one another's ends.
+// computing thread each) with bulk asynchronous copies.  Pass 1 keeps a running maximum (over whole chunks the warp's) and a
+// sum per lane; the warps' (maximum, sum) pairs meet once, in shared memory or in distributed shared memory across the
+// cluster.  Pass 2 turns the row into its gradient: first the last chunks, which are still in the ring, then the others,
+// which come through the ring again from L2, the last one first.  Copies that will be wanted again ask L2 to keep them
+// (evict_last), the others let go (evict_first).  CTAs are not persistent: the hardware deals rows to SMs as they come free,
+// which rows that are out make uneven, and co-resident CTAs cover one another's ends.
 //
 // Measured on 4096 x 131072 bf16 logits, single launches / back to back at the power cap, of the measured copy bandwidth:
 // the log-probability alone 0.97 / 0.92, with its gradient 0.90 / 0.84.  Without the L2 hints half of pass 2's reads miss L2:
@@ -118,8 +118,8 @@ __device__ __forceinline__ uint4 minus_infinity() {
   return make_uint4(w, w, w, w);
 }
 
-// A sum of 2^((x - m) c) known by its reference m and its value s.  The reference is any value not far below the
-// largest x: -infinity while nothing but -infinity has been seen.
+// A sum of 2^((x - m) c) known by the largest x, m, and its value s.  m is -infinity while nothing but -infinity has
+// been seen.
 struct Sum {
   float m, s;
 };
@@ -130,18 +130,21 @@ __device__ __forceinline__ Sum warp_join(Sum v, float c) {
   return {m, warp_allreduce<SumOp>(v.s)};
 }
 
-// The sum a lane keeps while it walks a row: two pairs of partial sums of 2^((x + nm) c), nm = -(its reference).
+// The sum a lane keeps while it walks a row: two pairs of partial sums of 2^((x + nm) c), nm = -(its largest x).
 struct Walk {
   float m, nm;
   F2 s0, s1;
 };
-// NV vectors into the sum.  The reference moves only when their maximum exceeds it by a factor of 2^24, which the
-// partial sums bear; the first vectors that are not all -infinity set it.
-template <typename T, int NV>
-__device__ __forceinline__ void walk(const uint4 (&u)[NV], float c, float margin, Walk& k) {
+// NV vectors into the sum.  The reference is the maximum itself, moved as soon as it is exceeded: a token that the model
+// is sure of then has 2^0 = 1 exactly in a sum little above 1, and its log-probability, near 0, keeps its digits.  (Moved
+// only when exceeded by 2^24, the logarithm was the small difference of two numbers near 24, 2e-6 off.)
+// WARP: all lanes are here and take the warp's maximum, which moves seldom (128 x 131072 bf16 forward 10.7 us, 10.9 with a
+// maximum per lane, 10.4 with the reference left behind); otherwise a lane its own.
+template <typename T, int NV, bool WARP>
+__device__ __forceinline__ void walk(const uint4 (&u)[NV], float c, Walk& k) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(u);
-  const float top   = words_max<T, 4 * NV>(w);
-  if (top > k.m + margin) {
+  const float top   = WARP ? warp_max(words_max<T, 4 * NV>(w)) : words_max<T, 4 * NV>(w);
+  if (top > k.m) {
     const float f = ex2((k.m - top) * c);
     k.s0          = mul2(k.s0, pair(f, f));
     k.s1          = mul2(k.s1, pair(f, f));
@@ -261,18 +264,18 @@ struct Call {
   T* out_grad;
   int cols, entries, wide, teacher;
   float weight_value;
-  float inv_t, c, margin;  // 1 / temperature; the exponentials are 2^(c (x - reference)); by how much that moves at once
+  float inv_t, c;  // 1 / temperature; the exponentials are 2^(c (x - largest x))
   Policy policy;
 };
 #define ROW_LOSS_PARAMS                                                                                                  \
   const T *__restrict__ x, const void *__restrict__ ids, const void *__restrict__ a0, const float *__restrict__ a1,       \
       const float *__restrict__ a2, const float *__restrict__ weight, float *__restrict__ out_loss,                       \
       float *__restrict__ out_lp, T *__restrict__ out_grad, long long rows, long long cols, long long entries,            \
-      long long wide, long long teacher, double weight_value, double inv_t, double c, double margin, double clip_low,     \
-      double clip_high, double kl_coef
+      long long wide, long long teacher, double weight_value, double inv_t, double c, double clip_low, double clip_high,   \
+      double kl_coef
 #define ROW_LOSS_CALL                                                                                                    \
   {x, ids, a0, a1, a2, weight, out_loss, out_lp, out_grad, (int)cols, (int)entries, (int)wide, (int)teacher,              \
-   (float)weight_value, (float)inv_t, (float)c, (float)margin, {(float)clip_low, (float)clip_high, (float)kl_coef}}
+   (float)weight_value, (float)inv_t, (float)c, {(float)clip_low, (float)clip_high, (float)kl_coef}}
 
 // What a row's scalar operands say.
 struct Head {
@@ -372,8 +375,8 @@ template <typename T, int KIND>
 __device__ __forceinline__ Terms row_terms(const Call<T>& o, long long row, const Head& h, const Sum& t, float xa,
                                            const PolicyOperands& po, const Kept& kept, bool writes, bool sums, int lane) {
   Terms k        = {-finite_ref(t.m), t.s, h.w, 0.0f, -INFINITY, 0.0f, h.live};
-  const float lg = log2f(t.s);
-  auto logq      = [&](float v) { return ((v + k.nm) * o.c - lg) * 0.6931471805599453f; };
+  const float lg = logf(t.s);
+  auto logq      = [&](float v) { return fmaf(v + k.nm, o.inv_t, -lg); };
   float loss     = 0.0f;
   if (KIND != kDistill) {
     const float lp = logq(xa);
@@ -399,10 +402,10 @@ __device__ __forceinline__ Terms row_terms(const Call<T>& o, long long row, cons
   for (int n = lane; n < o.entries && k.live; n += 32) k.tsum += ex2((kept.t[n] - k.tmax) * o.c);
   k.tsum = warp_allreduce<SumOp>(k.tsum);
   if (o.out_loss && sums) {
-    const float lt = log2f(k.tsum);
+    const float lt = logf(k.tsum);
     for (int n = lane; n < o.entries && k.live; n += 32) {
-      const float lp2 = (kept.t[n] - k.tmax) * o.c - lt, p = ex2(lp2);
-      if (p != 0.0f) loss += p * (lp2 * 0.6931471805599453f - logq(kept.x[n]));
+      const float d = kept.t[n] - k.tmax, p = __fdividef(ex2(d * o.c), k.tsum);
+      if (p != 0.0f) loss += p * (fmaf(d, o.inv_t, -lt) - logq(kept.x[n]));
     }
     loss = warp_allreduce<SumOp>(loss);
     if (lane == 0) o.out_loss[row] = k.live ? h.w * loss : 0.0f;
@@ -434,7 +437,8 @@ template <typename T, int KIND, class Mine>
 __device__ __forceinline__ void special_columns(const Call<T>& o, T* gr, const Terms& k, const Head& h, float xa,
                                                 const Kept& kept, int lane, Mine mine) {
   if (KIND != kDistill) {
-    if (k.live && lane == 0 && mine(h.a)) Io<T>::store1(gr + h.a, k.slope * o.inv_t * (1.0f - __fdividef(ex2((xa + k.nm) * o.c), k.S)));
+    // 1 - q as (S - e) / S: a difference of near numbers is exact.
+    if (k.live && lane == 0 && mine(h.a)) Io<T>::store1(gr + h.a, k.slope * o.inv_t * __fdividef(k.S - ex2((xa + k.nm) * o.c), k.S));
   } else if (k.live) {
     const float it = 1.0f / k.tsum;
     for (int n = lane; n < o.entries; n += 32) {
@@ -623,11 +627,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
       uint4 u[kUnroll];
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j) u[j] = src[j * T32];
-      walk<T, kUnroll>(u, o.c, o.margin, k);
+      walk<T, kUnroll, true>(u, o.c, k);
     } else {
       for (int j = tid; j < left; j += T32) {
         const uint4 u[1] = {src[j - tid]};
-        walk<T, 1>(u, o.c, o.margin, k);
+        walk<T, 1, false>(u, o.c, k);
       }
     }
     if (i < chunks - held) leave(slot);
@@ -761,10 +765,10 @@ __global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOS
   }
   Walk k = start_walk(xe, o.c);
   if constexpr (NV == 8) {
-    walk<T, 4>(reinterpret_cast<const uint4(&)[4]>(u[0]), o.c, o.margin, k);
-    walk<T, 4>(reinterpret_cast<const uint4(&)[4]>(u[4]), o.c, o.margin, k);
+    walk<T, 4, false>(reinterpret_cast<const uint4(&)[4]>(u[0]), o.c, k);
+    walk<T, 4, false>(reinterpret_cast<const uint4(&)[4]>(u[4]), o.c, k);
   } else {
-    walk<T, NV>(u, o.c, o.margin, k);
+    walk<T, NV, false>(u, o.c, k);
   }
   Sum t = end_walk(k, o.c);
   if (KIND == kDistill && o.entries <= T32) keep_entry(kept, tid, entry);
@@ -800,10 +804,10 @@ __global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOS
 }  // namespace
 
 #define REG_ROW_LOSS(KNAME, KIND, GNAME, GRAD, TNAME, T)                                                                      \
-  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME, 22, kMaxWarps * 32 + 32, k_row_loss<T, KIND, GRAD>);         \
-  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n2", 22, 256, k_row_loss_short<T, KIND, GRAD, 2>);          \
-  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n4", 22, 256, k_row_loss_short<T, KIND, GRAD, 4>);          \
-  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n8", 22, 256, k_row_loss_short<T, KIND, GRAD, 8>)
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME, 21, kMaxWarps * 32 + 32, k_row_loss<T, KIND, GRAD>);         \
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n2", 21, 256, k_row_loss_short<T, KIND, GRAD, 2>);          \
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n4", 21, 256, k_row_loss_short<T, KIND, GRAD, 4>);          \
+  CINN_B200_REGISTER_KERNEL_PDL("row_loss_" KNAME GNAME "_" TNAME "_n8", 21, 256, k_row_loss_short<T, KIND, GRAD, 8>)
 #define REG_ROW_LOSS_KINDS(TNAME, T)                           \
   REG_ROW_LOSS("logprob", kLogprob, "", false, TNAME, T);      \
   REG_ROW_LOSS("logprob", kLogprob, "_grad", true, TNAME, T);  \
