@@ -175,6 +175,23 @@ static int LaunchKernel(const void* kernel_fn, void* v_args, int num_args, int g
   return LaunchEntry(entry, v_args, num_args, gx, gy, gz, bx, by, bz, cluster_x, dyn_smem, stream);
 }
 
+// Lets `kernel_fn` be launched on the current device with this much dynamic shared memory.  One kernel serves plans of
+// several sizes, and host threads launch them side by side: the limit only ever rises, so that none is refused because
+// another asked for less between its own call here and its launch.
+static cudaError_t RaiseSharedMemoryLimit(const void* kernel_fn, size_t bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, size_t> limits;  // kernel, device -> what it may take
+  int dev       = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  size_t& limit = limits[{kernel_fn, dev}];
+  if (bytes <= limit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel_fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) limit = bytes;
+  return e;
+}
+
 // Group entry points already hold the table entry and come straight here.
 static int LaunchEntry(const KernelEntry* entry, void* v_args, int num_args, int gx, int gy, int gz, int bx, int by,
                        int bz, unsigned cluster_x, size_t dyn_smem, void* stream) {
@@ -198,7 +215,7 @@ static int LaunchEntry(const KernelEntry* entry, void* v_args, int num_args, int
     }
   }
   if (dyn_smem > 40 * 1024) {  // static + dynamic above 48 KiB needs the opt-in
-    cudaError_t e = cudaFuncSetAttribute(kernel_fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dyn_smem);
+    cudaError_t e = RaiseSharedMemoryLimit(kernel_fn, dyn_smem);
     if (e != cudaSuccess)
       return SetError(CINN_B200_ECUDA, "kernel %s: cannot reserve %zu bytes of shared memory: %s", entry->name,
                       dyn_smem, cudaGetErrorString(e));
