@@ -228,6 +228,14 @@ struct LossMatcher {
     return a;
   }
   static double Attr(const OpDesc& op, const char* key) { return atof(op.attrs.at(key).c_str()); }
+  // Whether two ops were given the same parameters, by value: one may spell out a default, or write 1 as 1.0.
+  static bool SameParameters(const OpDesc& a, const OpDesc& b) {
+    for (const char* key : {"temperature", "clip_low", "clip_high", "kl_coef"}) {
+      if (a.attrs.count(key) != b.attrs.count(key)) return false;
+      if (a.attrs.count(key) && Attr(a, key) != Attr(b, key)) return false;
+    }
+    return true;
+  }
   const TensorDesc& Input(const std::string& value) const { return g.inputs[input_index.at(value)]; }
   // The value of a per-row factor that is one constant (its pointer is null then).
   ArgSpec Constant(const std::string& value) const {
@@ -307,7 +315,7 @@ struct LossMatcher {
   // kind 0 token_logprob, 1 policy, 2 distill; any of the three results may be absent.
   std::unique_ptr<CompiledGroup> PlanRows(int kind, const OpDesc* loss, const OpDesc* grad, const OpDesc* logprob) {
     const OpDesc& main = grad ? *grad : loss ? *loss : *logprob;
-    if (loss && grad && (loss->inputs != grad->inputs || loss->attrs != grad->attrs))
+    if (loss && grad && (loss->inputs != grad->inputs || !SameParameters(*loss, *grad)))
       return Fail("the loss and its gradient differ in an operand or an attribute");
     if (logprob && (logprob->inputs[0] != main.inputs[0] || logprob->inputs[1] != main.inputs[1] ||
                     Attr(*logprob, "temperature") != Attr(main, "temperature")))

@@ -69,6 +69,39 @@ def test_ops_over_one_tensor_of_logits_share_a_kernel():
         assert sorted(plan(b)) == groups
 
 
+@pytest.mark.parametrize("given", [{}, {"clip_low": 0.2}, {"kl_coef": 0, "clip_high": "2e-1"}, {"temperature": "1.00"}])
+def test_parameters_are_compared_by_value(given):
+    """One op on defaults or with numbers written another way, the other with the values spelled out."""
+    b, v = net_with()
+    b.policy_loss(*policy_args(v))
+    b._op("policy_loss_grad", policy_args(v), **given)
+    assert plan(b) == ["row_loss"]
+    b, v = net_with()
+    b._op("distill_loss", [v["x"], v["t"], v["i"], v["w"]])
+    b.distill_loss_grad(v["x"], v["t"], v["i"], v["w"], temperature=1)
+    assert plan(b) == ["row_loss"]
+
+
+@pytest.mark.parametrize("one,two,good", [("temperature=1", "temperature=1.0", True), ("", "temperature=1", True),
+                                          ("kl_coef=0.5", "kl_coef=5e-1", True), ("temperature=1", "temperature=2", False),
+                                          ("", "kl_coef=0.1", False)])
+def test_parameters_of_a_group_description_are_compared_by_value(one, two, good):
+    text = """group fn_by_value
+input x float32 4,50
+input a int64 4
+input w float32 4
+op policy_loss l = x a w w w w ; %s
+op policy_loss_grad d = x a w w w w ; %s
+output l float32 4
+output d float32 4,50
+""" % (one, two)
+    if good:
+        cinn_b200.FusedGroup(text).release()
+    else:
+        with pytest.raises(CinnB200Error, match="differ in an operand or an attribute"):
+            cinn_b200.FusedGroup(text)
+
+
 def test_ops_that_differ_stay_apart():
     b, v = net_with()
     b.policy_loss(*policy_args(v), kl_coef=0.1)
