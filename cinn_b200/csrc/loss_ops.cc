@@ -243,6 +243,14 @@ struct LossMatcher {
     return F(it == constants.end() ? 0.0 : it->second);
   }
 
+  // The reference policy's log-probabilities where there is no KL term: they are not read (the kernel gets a null pointer
+  // for a constant, and its weight of the term as float32).
+  static bool IsPlaceholder(const OpDesc& op, size_t operand) {
+    if (operand != 3 || (op.type != "policy_loss" && op.type != "policy_loss_grad")) return false;
+    double kl = 0.0;
+    return !op.attrs.count("kl_coef") || (ReadNumber(op.attrs, "kl_coef", &kl) && (float)kl == 0.0f);
+  }
+
   std::unique_ptr<CompiledGroup> Run() {
     std::map<std::string, OpDesc> ops;  // by type, attributes completed
     std::map<std::string, TensorDesc> fills;
@@ -270,8 +278,8 @@ struct LossMatcher {
       for (size_t k = 0; k < op.inputs.size(); ++k) {
         const std::string& v = op.inputs[k];
         if (fills.count(v)) {
-          if ((int)k != FindSpec(op.type)->weight)
-            return Fail(op.type + ": operand '" + v + "' is a constant, which only the per-row weight may be");
+          if ((int)k != FindSpec(op.type)->weight && !IsPlaceholder(op, k))
+            return Fail(op.type + ": operand '" + v + "' is a constant, which only the per-row weight may be (and ref_logprob while kl_coef is 0)");
           in.push_back(fills[v]);
           continue;
         }

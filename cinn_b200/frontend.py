@@ -389,8 +389,9 @@ class NetBuilder:
     # ---- losses over rows of logits, and their gradients ------------------------------------------------
     # `logits` is [rows..., columns] in float32 / float16 / bfloat16; ids are int32 / int64; everything with one value
     # per row (rows...) is float32.  A row whose `weight` is 0 is out: loss 0 and a gradient row of zeros, whatever
-    # else it holds.  `weight` (and `dlogprob`) may be a fill_constant.  A gradient is that of the SUM of the losses;
-    # scale it through the weight.  The ops over one tensor of logits run as one kernel that reads it once.
+    # else it holds.  `weight` (and `dlogprob`) may be a fill_constant; no other operand may, which compiling the program
+    # says (`ref_logprob` may while kl_coef is 0).  A gradient is that of the SUM of the losses; scale it through the
+    # weight.  The ops over one tensor of logits run as one kernel that reads it once.
     def token_logprob(self, logits, target, temperature=1.0):
         """log softmax(logits / temperature)[target], float32; 0 where the target lies outside [0, columns)."""
         return self._op("token_logprob", [logits, target], temperature=float(temperature))
@@ -405,7 +406,7 @@ class NetBuilder:
         """Clipped policy loss per token, with the KL term against a reference policy: with lp = log
         softmax(logits / temperature)[action], r = exp(lp - old_logprob) and gap = ref_logprob - lp,
         weight * (kl_coef * (exp(gap) - gap - 1) - min(r * advantage, clip(r, 1 - clip_low, 1 + clip_high) * advantage)).
-        With kl_coef 0 the reference's log-probabilities are not read.  float32."""
+        With kl_coef 0 the reference's log-probabilities are not read: a fill_constant will do.  float32."""
         return self._op("policy_loss", [logits, action, old_logprob, ref_logprob, advantage, weight],
                         clip_low=float(clip_low), clip_high=float(clip_high), kl_coef=float(kl_coef),
                         temperature=float(temperature))

@@ -152,7 +152,8 @@ int cinn_b200_group_host_chunks(const char* fn_name);
  *     expert_counts       index[tokens..., slots] weight        ; num_experts    int32 [num_experts <= 1024]
  *     balance_loss[_grad] x counts weight        E sum_e counts_e / sum(counts) sum_t weight_t softmax(x_t)_e, E <= 1024 columns
  * A row of weight 0, or whose token id lies outside the columns, is out: its loss is 0 and its gradient row 0 whatever
- * else it holds.  The weight (and dlogprob) may be a fill_constant.  Gradients smaller than 2^-126 may come back as 0.
+ * else it holds.  The weight (and dlogprob), and ref while kl_coef is 0, may be a fill_constant; no
+ * other operand may.  Gradients smaller than 2^-126 may come back as 0.
  */
 typedef struct cinn_b200_builder cinn_b200_builder;
 cinn_b200_builder* cinn_b200_builder_create(const char* name);

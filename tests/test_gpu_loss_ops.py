@@ -464,6 +464,21 @@ def test_policy_without_kl_reads_no_reference():
     assert torch.isfinite(got["loss"]).all() and torch.isfinite(got["dx"]).all()
 
 
+@pytest.mark.parametrize("cols", [301, 3001, 40000])
+def test_a_constant_in_place_of_a_reference_that_is_not_read(cols):
+    g, x, a = make(5, cols, "float32")
+    inputs = policy_inputs(g, x, a)
+
+    def build(constant):
+        def f(b, v):
+            ref = b.fill_constant([5], 0.0) if constant else v["ref"]
+            args = [v["x"], v["a"], v["old"], ref, v["adv"], v["w"]]
+            return {"loss": b.policy_loss(*args), "dx": b.policy_loss_grad(*args)}
+        return f
+    one, two = run_program(build(False), inputs, want_groups=1), run_program(build(True), inputs, want_groups=1)
+    assert torch.equal(one["loss"], two["loss"]) and torch.equal(one["dx"], two["dx"])
+
+
 def test_balance_without_any_choice_and_without_any_token():
     x = torch.randn(9, 12, device="cuda")
     i = torch.full((9, 2), -1, device="cuda")

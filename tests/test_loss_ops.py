@@ -151,6 +151,23 @@ def test_a_constant_weight_is_taken_and_other_constants_are_refused():
         plan(b)
 
 
+def test_a_reference_that_is_not_read_may_be_a_constant():
+    for kl in (0.0, 1e-60):  # the kernel's weight of the term is a float32
+        b, v = net_with()
+        args = policy_args(v)
+        args[3] = b.fill_constant([6], 0.0)
+        b.policy_loss(*args, kl_coef=kl)
+        b.policy_loss_grad(*args, kl_coef=kl)
+        assert plan(b) == ["row_loss"]
+    b, v = net_with()
+    b.policy_loss(v["x"], v["a"], v["old"], b.fill_constant([6], 0.0), v["adv"], v["w"], kl_coef=0.1)
+    with pytest.raises(CinnB200Error, match="only the per-row weight"):
+        plan(b)
+    b, v = net_with()  # its shape and type are still checked
+    with pytest.raises(CinnB200Error, match="one value per row"):
+        b.policy_loss(v["x"], v["a"], v["old"], b.fill_constant([7], 0.0), v["adv"], v["w"])
+
+
 def test_export_and_load_keep_the_plan():
     b, v = net_with(dtype="bfloat16")
     b.policy_loss(*policy_args(v), kl_coef=0.1, clip_high=0.28)
