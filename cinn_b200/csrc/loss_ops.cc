@@ -254,6 +254,7 @@ struct LossMatcher {
   std::unique_ptr<CompiledGroup> Run() {
     std::map<std::string, OpDesc> ops;  // by type, attributes completed
     std::map<std::string, TensorDesc> fills;
+    std::set<std::string> written;
     for (auto& op : g.ops) {
       if (op.type != "fill_constant") continue;
       TensorDesc t;
@@ -274,6 +275,7 @@ struct LossMatcher {
       if (op.type == "fill_constant") continue;
       if (!IsLossOp(op.type)) return Fail("a loss op and '" + op.type + "' have no common kernel");
       if (ops.count(op.type)) return Fail("two " + op.type + " ops have no common kernel");
+      if (!written.insert(op.output).second) return Fail("two ops write '" + op.output + "'");
       std::vector<TensorDesc> in;
       for (size_t k = 0; k < op.inputs.size(); ++k) {
         const std::string& v = op.inputs[k];

@@ -242,6 +242,20 @@ def test_a_group_description_must_declare_the_result(dtype, shape, good):
             cinn_b200.FusedGroup(text)
 
 
+def test_a_group_in_which_two_ops_write_one_result_is_refused():
+    text = """group fn_one_result
+input x float32 4,50
+input a int64 4
+input w float32 4
+op policy_loss l = x a w w w w
+op token_logprob l = x a
+output l float32 4
+output p float32 4
+"""  # p would be written by no op
+    with pytest.raises(CinnB200Error, match="two ops write 'l'"):
+        cinn_b200.FusedGroup(text)
+
+
 def test_a_group_that_mixes_a_loss_with_another_op_is_refused():
     text = GROUP.format(name="mixed", dtype="float32", shape="4,50").replace(
         "output d", "op relu r = d\noutput d").replace("output d float32 4,50", "output d float32 4,50\noutput r float32 4,50")
