@@ -106,7 +106,7 @@ bool InferLossOp(const std::string& op, const std::vector<TensorDesc>& in, std::
     }
     return true;
   };
-  auto positive     = [](double v) { return v >= 1e-4 && v <= 1e4; };
+  auto positive     = [](double v) { return (float)v >= 1e-4f && (float)v <= 1e4f; };  // (1e-4f lies below 1e-4)
   auto non_negative = [](double v) { return v >= 0.0; };
   auto fraction     = [](double v) { return v >= 0.0 && v <= 1.0; };
 

@@ -211,6 +211,19 @@ def test_refusals(name, call, message):
         call(b, v)
 
 
+@pytest.mark.parametrize("text,good", [("0.0001", True), ("9.99999975e-05", True), ("10000", True), ("9e-05", False), ("10002", False),
+                                       ("-1", False), ("inf", False), ("1x", False)])
+def test_borders_of_the_temperature(text, good):
+    """9.99999975e-05 is 1e-4 as a float, which the C++ front end passes on."""
+    b, v = net_with()
+    if good:
+        b._op("token_logprob", [v["x"], v["a"]], temperature=text)
+        assert plan(b) == ["row_loss"]
+    else:
+        with pytest.raises(CinnB200Error, match="temperature"):
+            b._op("token_logprob", [v["x"], v["a"]], temperature=text)
+
+
 def test_too_many_teacher_entries_or_columns_are_refused():
     b, v = net_with(k=1025, cols=4000)
     with pytest.raises(CinnB200Error, match="1024 teacher entries"):
