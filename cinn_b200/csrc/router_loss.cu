@@ -17,41 +17,13 @@
 #include <type_traits>
 #include "device_math.cuh"
 #include "kernel_registry.h"
+#include "pair_math.cuh"
 
 namespace cinn_b200 {
 namespace {
 
 constexpr int kRouterThreads = 512;
 constexpr int kMaxExperts    = 1024;
-
-// Pairs of floats in one 64-bit register, for the two-wide arithmetic of sm_100.
-typedef unsigned long long F2;
-__device__ __forceinline__ F2 pair(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpair(F2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 
 // What a lane loads at once: a vector of V elements, or one element (V = 1).
 template <typename T, int V>
@@ -219,13 +191,6 @@ __global__ void __launch_bounds__(V * NV > 16 ? kRouterThreads / 2 : kRouterThre
   if (!out_part) return;
   sum = cta_allreduce<SumOp>(sum, scratch);
   if (threadIdx.x == 0) out_part[blockIdx.x] = (float)cols * sum;
-}
-
-// All warps of the cluster, each of them together.
-__device__ __forceinline__ void cluster_barrier() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Adds this thread's choices to the CTA's bins, eight read before the first is counted (compared as they come, each load

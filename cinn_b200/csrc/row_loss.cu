@@ -35,6 +35,7 @@
 // barriers it shares with others; the copying lane waits for all its copies, bounded, before it leaves.
 #include "device_math.cuh"
 #include "kernel_registry.h"
+#include "pair_math.cuh"
 #include "tma_utils.cuh"
 
 namespace cinn_b200 {
@@ -56,29 +57,6 @@ __device__ __forceinline__ float load_float(const void* p, long long i, int type
   return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-// Pairs of floats in one 64-bit register, for the two-wide arithmetic of sm_100.
-typedef unsigned long long F2;
-__device__ __forceinline__ F2 pair(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpair(F2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float warp_max(float v) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -225,12 +203,6 @@ __device__ __forceinline__ unsigned sm_count() {
   unsigned n;
   asm("mov.u32 %0, %%nsmid;" : "=r"(n));
   return n;
-}
-// All warps of the cluster, each of them together.
-__device__ __forceinline__ void cluster_barrier() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Where a row's vectors lie: `head` elements in front of the first 16-byte boundary, `nvec` vectors, `tail` elements;
 // and this CTA's stretch of the vectors, `count` from `start` on (`per` to a CTA).
