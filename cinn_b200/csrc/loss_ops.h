@@ -15,7 +15,8 @@
 namespace cinn_b200 {
 
 // token_logprob, token_logprob_grad, policy_loss, policy_loss_grad, distill_loss, distill_loss_grad, expert_counts,
-// balance_part, balance_loss_grad.  (balance_loss is balance_part followed by reduce_sum.)
+// balance_part, balance_loss_grad.  (balance_loss is balance_part, followed by reduce_sum where the tokens make more than
+// one part.)
 bool IsLossOp(const std::string& op_type);
 
 // Checks the operands and attributes of one loss op, fills in default attributes and the result's type and shape.

@@ -10,8 +10,8 @@
 // weight 0 is out: it adds nothing and is not read, and its gradient row is 0.
 //
 // Bound by HBM for long batches and, at these row lengths, by instructions nearly as much: three reductions over a token's
-// lanes for eight elements per lane.  Measured with counts, loss and gradient, 65536 x 256 fp32, 8 choices: 28 us (119 MB,
-// 0.65 of the copy bandwidth), of which 6 us are the three small launches around this kernel; 480 us before the row lay
+// lanes for eight elements per lane.  Measured with counts, loss and gradient, 65536 x 256 fp32, 8 choices: 29 us (119 MB,
+// 0.63 of the copy bandwidth), of which 6 us are the three small launches around this kernel; 480 us before the row lay
 // in registers as vectors, 34 with 16 elements per lane, 32 with column sums (which the loss does not need) kept too, 33 with two tokens
 // per trip (84 registers: one CTA per SM).
 #include <type_traits>

@@ -24,9 +24,9 @@
 // (evict_last), the others let go (evict_first).  CTAs are not persistent: the hardware deals rows to SMs as they come free,
 // which rows that are out make uneven, and co-resident CTAs cover one another's ends.
 //
-// Measured on 4096 x 131072 bf16 logits, single launches / back to back at the power cap, of the measured copy bandwidth:
-// the log-probability alone 0.97 / 0.92, with its gradient 0.90 / 0.84.  Without the L2 hints half of pass 2's reads miss L2:
-// 0.76.  4 slots of 8 warps against 3 / 6 slots: level on long rows, 0.64 against 0.64 / 0.55 at 1000 x 50021 fp16; 16 warps
+// Measured on 4096 x 131072 bf16 logits back to back at the power cap, of the measured copy bandwidth: the log-probability
+// alone 0.91 to 0.97 (GPUs differ), with the gradient 0.82 to 0.85.  Variants of the latter, single launches, 0.90 as
+// built: without the L2 hints half of pass 2's reads miss L2, 0.76.  4 slots of 8 warps against 3 / 6 slots: level on long rows, 0.64 against 0.64 / 0.55 at 1000 x 50021 fp16; 16 warps
 // 0.78, 4 warps 0.80.  Pass 2 without the chunks that are still there 0.825.  The row held on chip by a cluster of 2 or 4
 // CTAs: 0.68; rings in clusters of 2 / 4: 0.80 / 0.74.  Persistent CTAs that fetch the next row ahead, rows dealt statically
 // or by cluster launch control: 0.75, 0.77.  Plain loads into registers: 0.81.
@@ -162,7 +162,9 @@ __device__ __forceinline__ void common_part(uint4 (&u)[NV], float nm, float c, f
 struct Policy {
   float lo, hi, kl;  // clip bounds of the ratio (1 - clip_low, 1 + clip_high), weight of the KL term
 };
-// The policy loss of one token (without its weight) and its derivative with respect to the log-probability.
+// The policy loss of one token (without its weight) and its derivative with respect to the log-probability.  In float32: old
+// and ref come as float32 log-probabilities, off by half a step each, which moves ratio and gap as much as lp's own
+// rounding does; wider arithmetic behind them would add no digits.
 __device__ __forceinline__ void policy_terms(float lp, float old, float ref, float adv, const Policy& c, float* loss,
                                              float* slope) {
   const float r = expf(lp - old), free = r * adv, held = fminf(fmaxf(r, c.lo), c.hi) * adv;

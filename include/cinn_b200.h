@@ -152,8 +152,9 @@ int cinn_b200_group_host_chunks(const char* fn_name);
  *     expert_counts       index[tokens..., slots] weight        ; num_experts    int32 [num_experts <= 1024]
  *     balance_loss[_grad] x counts weight        E sum_e counts_e / sum(counts) sum_t weight_t softmax(x_t)_e, E <= 1024 columns
  * A row of weight 0, or whose token id lies outside the columns, is out: its loss is 0 and its gradient row 0 whatever
- * else it holds.  The weight (and dlogprob), and ref while kl_coef is 0, may be a fill_constant; no
- * other operand may.  Gradients smaller than 2^-126 may come back as 0.
+ * else it holds.  The weight (and dlogprob), and ref while kl_coef is 0, may be a fill_constant; no other operand may.
+ * temperature is 1e-4 to 1e4, clip_low 0 to 1, clip_high and kl_coef 0 or more; every extent is at least 1; a result's buffer
+ * is no operand's.  Gradients smaller than 2^-126 may come back as 0.
  */
 typedef struct cinn_b200_builder cinn_b200_builder;
 cinn_b200_builder* cinn_b200_builder_create(const char* name);

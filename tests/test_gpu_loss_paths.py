@@ -4,7 +4,9 @@ import pytest
 import torch
 
 import cinn_b200
-from tests.test_gpu_loss_ops import TYPES, U, check_grad, delta, distill64, distill_inputs, make, near, run_program
+from cinn_b200 import common, frontend
+from tests.test_gpu_loss_ops import (NAMES, POLICY, TYPES, U, check_grad, delta, distill64, distill_inputs, make, near,
+                                     policy_inputs, run_program)
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +102,51 @@ def test_host_buffers_in_chunks_of_rows(what):
     # another number of rows may share a row among more CTAs: sums of magnitudes up to 1 regrouped, and a loss of at most w (ln 4099 + 8)
     assert (got - out.cpu()).abs().max() <= 200 * U * (4 if what == "distill" else 1)
     group.release()
+
+
+def test_a_captured_program_of_the_row_losses_reads_the_inputs_of_each_replay():
+    """Long rows on clusters, long rows one CTA each and short rows, replayed without a wait while the inputs change."""
+    sizes = {"few": (6, 60000), "many": (450, 9000), "short": (70, 500)}
+    net = frontend.NetBuilder("captured_losses")
+    sets = [{} for _ in range(4)]
+    outs, v = [], {}
+    for n, (rows, cols) in sizes.items():
+        for seed, s in enumerate(sets):
+            g, x, a = make(rows, cols, "bfloat16", seed=seed)
+            p, t = policy_inputs(g, x, a), distill_inputs(g, x, 9)
+            p["w"] = p["w"].roll(seed)
+            s.update({n + k: q for k, q in {**p, "t": t["t"], "i": t["i"]}.items()})
+        for k in ("x", "a", "old", "ref", "adv", "w", "t", "i"):
+            q = sets[0][n + k]
+            v[k] = net.create_input(NAMES[q.dtype], list(q.shape), n + k)
+        args = [v[k] for k in ("x", "a", "old", "ref", "adv", "w")]
+        outs += [net.token_logprob(v["x"], v["a"]), net.policy_loss(*args, **POLICY), net.policy_loss_grad(*args, **POLICY),
+                 net.distill_loss(v["x"], v["t"], v["i"], v["w"]), net.distill_loss_grad(v["x"], v["t"], v["i"], v["w"])]
+    comp = frontend.Computation.build_and_compile(common.DefaultNVGPUTarget(), net, fetch=[str(o) for o in outs])
+    feed = {k: torch.empty_like(q) for k, q in sets[0].items()}
+    res = [torch.empty(o.shape, dtype=TYPES[o.type.name], device="cuda") for o in outs]
+    for k, q in feed.items():
+        comp.get_tensor(k).bind(q.data_ptr())
+    for o, q in zip(outs, res):
+        comp.get_tensor(str(o)).bind(q.data_ptr())
+    stream = torch.cuda.Stream()
+
+    def go(run, wait):
+        got = []
+        with torch.cuda.stream(stream):
+            for s in sets:
+                for k, q in feed.items():
+                    q.copy_(s[k])
+                run(stream.cuda_stream)
+                if wait:
+                    torch.cuda.synchronize()
+                got.append([q.clone() for q in res])
+        torch.cuda.synchronize()
+        return got
+    torch.cuda.synchronize()
+    want = go(comp.execute, True)
+    assert not torch.equal(want[0][2], want[1][2])
+    go(comp.execute_graph, True)  # captures
+    for _ in range(5):
+        for one, two in zip(go(comp.execute_graph, False), want):
+            assert all(torch.equal(p, q) for p, q in zip(one, two))
