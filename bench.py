@@ -219,6 +219,17 @@ def TORCH_OF_NUMPY(torch):
             np.dtype(np.bool_): torch.bool}
 
 
+def split_detail(line):
+    """The line to print, and what goes to stderr in full: sixty groups with their kernels and notes make a line of 20 KB,
+    which readers of its last kilobytes cannot parse.  The line keeps one figure per group (its fraction of the peak, or the
+    microseconds of a run where there is none) and the strong-scaling summary of its `config`."""
+    detail = {k: line[k] for k in ("groups", "strong_scaling_detail", "strong_scaling_emulated_detail") if k in line}
+    short = {k: v for k, v in line.items() if k not in detail}
+    if "groups" in detail:
+        short["groups"] = {n: g.get("frac_of_peak", g.get("us_per_run")) for n, g in detail["groups"].items()}
+    return short, detail
+
+
 def side_groups(torch, dev, peak, only=None):
     """Per-group throughput of the other fused groups (device-resident inputs, kernel time only)."""
     import cinn_b200
@@ -961,6 +972,9 @@ def main():
         dist.barrier()
         dist.destroy_process_group()
     if rank == 0:
+        line, detail = split_detail(line)
+        if detail:
+            print(json.dumps(detail), file=sys.stderr)
         print(json.dumps(line))
     return 0
 
