@@ -25,11 +25,12 @@
 // which rows that are out make uneven, and co-resident CTAs cover one another's ends.
 //
 // Measured on 4096 x 131072 bf16 logits back to back at the power cap, of the measured copy bandwidth: the log-probability
-// alone 0.91 to 0.97 (GPUs differ), with the gradient 0.82 to 0.85.  Variants of the latter, single launches, 0.90 as
-// built: without the L2 hints half of pass 2's reads miss L2, 0.76.  4 slots of 8 warps against 3 / 6 slots: level on long rows, 0.64 against 0.64 / 0.55 at 1000 x 50021 fp16; 16 warps
-// 0.78, 4 warps 0.80.  Pass 2 without the chunks that are still there 0.825.  The row held on chip by a cluster of 2 or 4
-// CTAs: 0.68; rings in clusters of 2 / 4: 0.80 / 0.74.  Persistent CTAs that fetch the next row ahead, rows dealt statically
-// or by cluster launch control: 0.75, 0.77.  Plain loads into registers: 0.81.
+// alone 0.91 to 0.97 (GPUs differ), with the gradient 0.82 to 0.85.  Variants of the latter, single launches on one GPU, 0.90
+// as built there: without the L2 hints half of pass 2's reads miss L2, 0.76.  4 slots of 8 warps against 3 / 6 slots: level
+// on long rows, 0.64 against 0.64 / 0.55 at 1000 x 50021 fp16; 16 warps 0.78, 4 warps 0.80.  Pass 2 without the chunks that
+// are still there 0.825.  The row held on chip by a cluster of 2 or 4 CTAs: 0.68; rings in clusters of 2 / 4: 0.80 / 0.74.
+// Persistent CTAs that fetch the next row ahead, rows dealt statically or by cluster launch control: 0.75, 0.77.  Plain loads
+// into registers: 0.81.
 //
 // Every wait on a copy is bounded: a warp that gives up records it (cinn_b200_device_status) and goes on through the
 // barriers it shares with others; the copying lane waits for all its copies, bounded, before it leaves.
