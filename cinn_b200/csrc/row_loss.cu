@@ -339,7 +339,9 @@ __device__ __forceinline__ void prefetch_entries(const Call<T>& o, long long row
   for (int b = thread * 128; b < o.entries * wt; b += threads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p1 + b));
 }
 
-// What follows from a row's sum: q_j = 2^(c (x_j + nm)) / S, the gradient's common part coef * q_j.
+// What follows from a row's sum: q_j = 2^(c (x_j + nm)) / S, the gradient's common part coef * q_j.  The divisions are few, one
+// or two to a thread and row, and rounded ones: the approximate one took the error of a float32 gradient, 777 x 50021,
+// from 4.2e-8 to 5e-8 (2-norm, a maximum-subtracted softmax in float32 2.7e-8), at the same times.
 struct Terms {
   float nm, S, slope, coef, tmax, tsum;
   bool live;
@@ -379,7 +381,7 @@ __device__ __forceinline__ Terms row_terms(const Call<T>& o, long long row, cons
   if (o.out_loss && sums) {
     const float lt = logf(k.tsum);
     for (int n = lane; n < o.entries && k.live; n += 32) {
-      const float d = kept.t[n] - k.tmax, p = __fdividef(ex2(d * o.c), k.tsum);
+      const float d = kept.t[n] - k.tmax, p = ex2(d * o.c) / k.tsum;
       if (p != 0.0f) loss += p * (fmaf(d, o.inv_t, -lt) - logq(kept.x[n]));
     }
     loss = warp_allreduce<SumOp>(loss);
@@ -413,12 +415,12 @@ __device__ __forceinline__ void special_columns(const Call<T>& o, T* gr, const T
                                                 const Kept& kept, int lane, Mine mine) {
   if (KIND != kDistill) {
     // 1 - q as (S - e) / S: a difference of near numbers is exact.
-    if (k.live && lane == 0 && mine(h.a)) Io<T>::store1(gr + h.a, k.slope * o.inv_t * __fdividef(k.S - ex2((xa + k.nm) * o.c), k.S));
+    if (k.live && lane == 0 && mine(h.a)) Io<T>::store1(gr + h.a, k.slope * o.inv_t * ((k.S - ex2((xa + k.nm) * o.c)) / k.S));
   } else if (k.live) {
     const float it = 1.0f / k.tsum;
     for (int n = lane; n < o.entries; n += 32) {
       const int id = kept.id[n];
-      if (id >= 0 && mine(id)) Io<T>::store1(gr + id, k.coef * (__fdividef(ex2((kept.x[n] + k.nm) * o.c), k.S) - kept.mass[n] * it));
+      if (id >= 0 && mine(id)) Io<T>::store1(gr + id, k.coef * (ex2((kept.x[n] + k.nm) * o.c) / k.S - kept.mass[n] * it));
     }
   }
 }
@@ -642,7 +644,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32 + 32, 3) k_row_loss(ROW_LOSS_PA
   if (GRAD) {
     if (KIND == kDistill) column_masses(kept, o.entries, m, o.c, tid, T32);
     // Pass 2: coef * q_j everywhere, then the few columns that have a term of their own.
-    const float q0 = __fdividef(m.coef, m.S);
+    const float q0 = m.coef / m.S;
     int there      = (chunks - held) % N;  // slot of the first chunk that is still there
     for (int i = 0; i < chunks; ++i) {
       const int at = (i < held ? chunks - held + i : chunks - 1 - i) * chunk, left = r.count - at;
@@ -757,7 +759,7 @@ __global__ void __launch_bounds__(256, NV == 8 ? 2 : 4) k_row_loss_short(ROW_LOS
   const Terms m = row_terms<T, KIND>(o, row, h, t, xa, po, kept, tid == 0, warp == W - 1, lane);
   if (!GRAD) return;
   if (KIND == kDistill) column_masses(kept, o.entries, m, o.c, tid, T32);
-  const float q0 = __fdividef(m.coef, m.S);
+  const float q0 = m.coef / m.S;
   if (m.live) {
     common_part<T, NV>(u, m.nm, o.c, q0);
   } else {
